@@ -26,8 +26,13 @@ OUT = ROOT / "distributed_pytorch_amd" / "_C.so"
 ARCH = "gfx950"
 # Per-file code generation options. Keeping MFMA accumulators in architectural VGPRs avoids the
 # v_accvgpr_read/write traffic that VALU work on accumulators (softmax rescale, dS) otherwise pays.
+_NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # plain fp32 instructions only
 EXTRA_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "paged_plan.hip": _NO_PACKED_FP32,
+    "paged_append.hip": _NO_PACKED_FP32,
+    "paged_attn.hip": _NO_PACKED_FP32,
+    "penalties.hip": _NO_PACKED_FP32,
 }
 # Sources that textually include another source (rebuilt when that one changes).
 EXTRA_DEPS = {

@@ -3,6 +3,7 @@
 // fault the GPU), allocates outputs through the caching allocator and forwards raw pointers
 // plus the current HIP stream to the launchers in kernels.h.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -1277,6 +1278,276 @@ void transpose_bf16_many(const Tensor& in_ptrs, const Tensor& out_ptrs, int64_t 
                            (int)C, cur_stream());
 }
 
+// ---------------------------------------------------------------------------------------
+// Paged KV cache and logit penalties. Lengths, tables and slots are only read on the device: what they say is bounded
+// there against the sizes checked here.
+int paged_type(const Tensor& t, const char* who) {
+  const auto ty = t.scalar_type();
+  TORCH_CHECK(ty == at::kBFloat16 || ty == at::kHalf || ty == at::kFloat, who, ": bf16, fp16 or fp32 tensors, not ", ty);
+  return ty == at::kBFloat16 ? dpa::kTypeBf16 : ty == at::kHalf ? dpa::kTypeHalf : dpa::kTypeFloat;
+}
+
+void check_int_vec(const Tensor& t, int64_t n, const Tensor& like, const char* who, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() &&
+                  (n < 0 || t.numel() == n),
+              who, ": ", name, " must be a contiguous int32 vector", n < 0 ? "" : " of the right length",
+              " on the device of the other arguments");
+}
+
+// [P, page, nkv, width] with unit inner stride and strides that stay inside the tensor
+void check_pages(const Tensor& t, const char* who, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 4 && t.size(1) >= 1 && t.size(2) >= 1 && t.size(3) >= 1 &&
+                  (t.stride(3) == 1 || t.size(3) == 1),
+              who, ": ", name, " must be [pages, page, kv heads, width] on the GPU with unit inner stride");
+  TORCH_CHECK(t.size(0) * t.size(1) < (int64_t(1) << 31), who, ": more than 2^31 rows in ", name);
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_plan(const Tensor& q_lens, const Tensor& ctx_lens, Tensor table,
+                                                              const Tensor& free_pages, const Tensor& free_count,
+                                                              int64_t page, int64_t tokens) {
+  const char* who = "paged_plan";
+  TORCH_CHECK(q_lens.is_cuda(), who, ": q_lens must live on the GPU");
+  check_int_vec(q_lens, -1, q_lens, who, "q_lens");
+  const int64_t R = q_lens.numel();
+  check_int_vec(ctx_lens, R, q_lens, who, "ctx_lens");
+  check_int_vec(free_pages, -1, q_lens, who, "free_pages");
+  check_int_vec(free_count, -1, q_lens, who, "free_count");
+  TORCH_CHECK(free_count.numel() >= 1, who, ": free_count holds the number of free pages in its first entry");
+  TORCH_CHECK(table.device() == q_lens.device() && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == R &&
+                  (table.size(1) <= 1 || table.stride(1) == 1) && (R <= 1 || table.stride(0) >= table.size(1)),
+              who, ": block_table must be int32 [requests, columns] with unit inner stride on the same device");
+  TORCH_CHECK(page >= 1 && page <= (1 << 20), who, ": page size must be in [1, 2^20], not ", page);
+  TORCH_CHECK(tokens >= 0 && tokens <= (1 << 29), who, ": num_tokens must be in [0, 2^29], not ", tokens);
+  TORCH_CHECK(R < (1 << 30) && table.size(1) < (1 << 30) && free_pages.numel() < (int64_t(1) << 31), who, ": too many requests or pages");
+  c10::DeviceGuard guard(q_lens.device());
+  const auto opt = q_lens.options();
+  Tensor cu_q = at::empty({R + 1}, opt), kv_lens = at::empty({R}, opt), positions = at::empty({tokens}, opt),
+         slots = at::empty({tokens}, opt), left = at::empty({2}, opt);
+  dpa::PagedPlanArgs a{};
+  a.q_lens = q_lens.data_ptr<int>();
+  a.ctx_lens = ctx_lens.data_ptr<int>();
+  a.table = table.data_ptr<int>();
+  a.table_ld = table.stride(0);
+  a.free_pages = free_pages.data_ptr<int>();
+  a.free_count = free_count.data_ptr<int>();
+  a.free_cap = (int)free_pages.numel();
+  a.R = (int)R;
+  a.M = (int)table.size(1);
+  a.page = (int)page;
+  a.tokens = (int)tokens;
+  a.by_page = dpa::make_fast_div((int)page);
+  a.cu_q = cu_q.data_ptr<int>();
+  a.kv_lens = kv_lens.data_ptr<int>();
+  a.positions = positions.data_ptr<int>();
+  a.slots = slots.data_ptr<int>();
+  a.free_left = left.data_ptr<int>();
+  dpa::paged_plan(a, cur_stream());
+  return {cu_q, kv_lens, positions, slots, left};
+}
+
+void paged_append(Tensor k_pages, Tensor v_pages, const Tensor& k, const Tensor& v, const Tensor& slots) {
+  const char* who = "paged_append";
+  check_pages(k_pages, who, "k_pages");
+  check_pages(v_pages, who, "v_pages");
+  const int64_t P = k_pages.size(0), page = k_pages.size(1), H = k_pages.size(2);
+  TORCH_CHECK(v_pages.size(0) == P && v_pages.size(1) == page && v_pages.size(2) == H && v_pages.device() == k_pages.device(),
+              who, ": k_pages and v_pages must agree in all but their width");
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.size(0) == v.size(0) && k.size(1) == H && v.size(1) == H &&
+                  k.size(2) == k_pages.size(3) && v.size(2) == v_pages.size(3),
+              who, ": the new rows must be [tokens, kv heads, width] of the pages' heads and widths");
+  for (const Tensor* t : {&k, &v, (const Tensor*)&v_pages}) {
+    TORCH_CHECK(t->device() == k_pages.device() && t->scalar_type() == k_pages.scalar_type() &&
+                    (t->stride(-1) == 1 || t->size(-1) == 1),
+                who, ": all tensors share a device and a type, with unit inner stride");
+  }
+  paged_type(k_pages, who);
+  at::assert_no_internal_overlap(k_pages);
+  at::assert_no_internal_overlap(v_pages);
+  at::assert_no_overlap(k_pages, v_pages);
+  check_int_vec(slots, k.size(0), k_pages, who, "slots");
+  TORCH_CHECK(k.size(0) < (1 << 30) && page <= (1 << 20) && H * (k.size(2) + v.size(2)) < (1 << 20), who, ": size out of range");
+  c10::DeviceGuard guard(k_pages.device());
+  dpa::PagedAppendArgs a{};
+  a.k_pages = k_pages.data_ptr();
+  a.v_pages = v_pages.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.slots = slots.data_ptr<int>();
+  a.kp_ps = k_pages.stride(0);
+  a.kp_rs = k_pages.stride(1);
+  a.kp_hs = k_pages.stride(2);
+  a.vp_ps = v_pages.stride(0);
+  a.vp_rs = v_pages.stride(1);
+  a.vp_hs = v_pages.stride(2);
+  a.k_ts = k.stride(0);
+  a.k_hs = k.stride(1);
+  a.v_ts = v.stride(0);
+  a.v_hs = v.stride(1);
+  a.N = (int)k.size(0);
+  a.nkv = (int)H;
+  a.dk = (int)k.size(2);
+  a.dv = (int)v.size(2);
+  a.pages = (int)P;
+  a.page = (int)page;
+  a.elem = (int)k.element_size();
+  a.by_page = dpa::make_fast_div((int)page);
+  dpa::paged_append(a, cur_stream());
+}
+
+// out given: it is filled, rows outside every sequence stay as they are, and nothing is returned; else the rows
+// outside every sequence are zero.
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu_q,
+                       const Tensor& kv_lens, double scale, int64_t window, int64_t max_q, const std::optional<Tensor>& out) {
+  const char* who = "paged_attention";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.size(1) >= 1 && (q.stride(2) == 1 || q.size(2) == 1), who,
+              ": q must be [tokens, heads, width] on the GPU with unit inner stride");
+  check_pages(k_pages, who, "k_pages");
+  check_pages(v_pages, who, "v_pages");
+  const int64_t N = q.size(0), nh = q.size(1), W = q.size(2), nkv = k_pages.size(2);
+  TORCH_CHECK(v_pages.sizes() == k_pages.sizes() && k_pages.size(3) == W && W >= 1 && W <= 256, who,
+              ": keys and values must share the queries' width, at most 256");
+  TORCH_CHECK(nh % nkv == 0, who, ": heads must be a multiple of the kv heads");
+  for (const Tensor* t : {&k_pages, &v_pages})
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == q.scalar_type(), who, ": all tensors share a device and a type");
+  const int type = paged_type(q, who);
+  TORCH_CHECK(cu_q.dim() == 1 && cu_q.numel() >= 1, who, ": cu_q holds requests + 1 entries");
+  const int64_t R = cu_q.numel() - 1;
+  check_int_vec(cu_q, R + 1, q, who, "cu_q");
+  check_int_vec(kv_lens, R, q, who, "kv_lens");
+  TORCH_CHECK(table.device() == q.device() && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == R &&
+                  (table.size(1) <= 1 || table.stride(1) == 1) && (R <= 1 || table.stride(0) >= 0),
+              who, ": block_table must be int32 [requests, columns] with unit inner stride on the same device");
+  TORCH_CHECK(table.size(1) * k_pages.size(1) < (int64_t(1) << 30) && k_pages.size(1) <= (1 << 20), who,
+              ": more than 2^30 rows per request");
+  TORCH_CHECK(N < (1 << 29) && R < (1 << 29) && N * nh < (int64_t(1) << 31), who, ": too many rows");
+  TORCH_CHECK(window >= 0 && window < (int64_t(1) << 31), who, ": window must be positive (0: none)");
+  TORCH_CHECK(max_q >= 0, who, ": max_q must not be negative");
+  TORCH_CHECK(std::isfinite(scale), who, ": scale must be finite");
+  c10::DeviceGuard guard(q.device());
+  Tensor o;
+  if (out.has_value()) {
+    o = *out;
+    TORCH_CHECK(o.device() == q.device() && o.scalar_type() == q.scalar_type() && o.sizes() == q.sizes() &&
+                    (o.stride(2) == 1 || W == 1),
+                who, ": out must look like q, with unit inner stride");
+    at::assert_no_internal_overlap(o);
+    at::assert_no_overlap(o, q);
+  } else {
+    o = at::empty({N, nh, W}, q.options());
+  }
+  dpa::PagedAttnArgs a{};
+  a.q = q.data_ptr();
+  a.k = k_pages.data_ptr();
+  a.v = v_pages.data_ptr();
+  a.o = o.data_ptr();
+  a.table = table.data_ptr<int>();
+  a.cu_q = cu_q.data_ptr<int>();
+  a.kv_lens = kv_lens.data_ptr<int>();
+  a.table_ld = table.stride(0);
+  a.q_ts = q.stride(0);
+  a.q_hs = q.stride(1);
+  a.o_ts = o.stride(0);
+  a.o_hs = o.stride(1);
+  a.k_ps = k_pages.stride(0);
+  a.k_rs = k_pages.stride(1);
+  a.k_hs = k_pages.stride(2);
+  a.v_ps = v_pages.stride(0);
+  a.v_rs = v_pages.stride(1);
+  a.v_hs = v_pages.stride(2);
+  a.N = (int)N;
+  a.R = (int)R;
+  a.M = (int)table.size(1);
+  a.nh = (int)nh;
+  a.nkv = (int)nkv;
+  a.width = (int)W;
+  a.pages = (int)k_pages.size(0);
+  a.page = (int)k_pages.size(1);
+  a.by_page = dpa::make_fast_div(a.page);
+  a.scale = (float)scale;
+  a.window = (int)window;
+  a.max_q = (int)std::min<int64_t>(max_q > 0 ? max_q : N, N);
+  a.type = type;
+  a.zero_rest = !out.has_value();
+  dpa::paged_attn(a, cur_stream());
+  return out.has_value() ? Tensor() : o;
+}
+
+Tensor penalize_logits(const Tensor& logits, const std::optional<Tensor>& tokens, const std::optional<Tensor>& prompt_lens,
+                       const std::optional<Tensor>& total_lens, const std::optional<Tensor>& repetition,
+                       const std::optional<Tensor>& presence, const std::optional<Tensor>& frequency, double repetition_v,
+                       double presence_v, double frequency_v, const std::optional<Tensor>& bias,
+                       const std::optional<Tensor>& allowed, const std::optional<Tensor>& out) {
+  const char* who = "penalize_logits";
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), who,
+              ": logits must be [rows, vocabulary] on the GPU with unit inner stride");
+  const int64_t R = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(R <= 65535 && V < (1 << 30), who, ": at most 65535 rows");
+  dpa::PenaltyArgs a{};
+  a.type = paged_type(logits, who);
+  auto per_row = [&](const std::optional<Tensor>& t, at::ScalarType ty, const char* name, int& stride) -> const void* {
+    stride = 0;
+    if (!t.has_value()) return nullptr;
+    TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == ty && t->dim() == 1 && t->is_contiguous() &&
+                    (t->numel() == R || t->numel() == 1),
+                who, ": ", name, " must be one ", ty, " value or one per row, on the logits' device");
+    stride = t->numel() == 1 ? 0 : 1;
+    return t->data_ptr();
+  };
+  a.prompt_lens = (const int*)per_row(prompt_lens, at::kInt, "prompt_lens", a.prompt_stride);
+  a.total_lens = (const int*)per_row(total_lens, at::kInt, "total_lens", a.total_stride);
+  a.repetition = (const float*)per_row(repetition, at::kFloat, "repetition", a.repetition_stride);
+  a.presence = (const float*)per_row(presence, at::kFloat, "presence", a.presence_stride);
+  a.frequency = (const float*)per_row(frequency, at::kFloat, "frequency", a.frequency_stride);
+  a.repetition_v = (float)repetition_v;
+  a.presence_v = (float)presence_v;
+  a.frequency_v = (float)frequency_v;
+  if (tokens.has_value()) {
+    TORCH_CHECK(tokens->device() == logits.device() && (tokens->scalar_type() == at::kLong || tokens->scalar_type() == at::kInt) &&
+                    tokens->dim() == 2 && tokens->size(0) == R && (tokens->stride(1) == 1 || tokens->size(1) <= 1) &&
+                    tokens->size(1) < (int64_t(1) << 30),
+                who, ": tokens must be int64 or int32 [rows, history] with unit inner stride on the logits' device");
+    a.tokens = tokens->data_ptr();
+    a.tokens64 = tokens->scalar_type() == at::kLong;
+    a.tokens_ld = tokens->stride(0);
+    a.L = (int)tokens->size(1);
+  }
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->size(-1) == V &&
+                    (bias->stride(-1) == 1 || V == 1) && (bias->dim() == 1 || (bias->dim() == 2 && bias->size(0) == R)),
+                who, ": bias must be fp32 [vocabulary] or [rows, vocabulary] with unit inner stride on the logits' device");
+    a.bias = bias->data_ptr<float>();
+    a.bias_ld = bias->dim() == 2 ? bias->stride(0) : 0;
+  }
+  if (allowed.has_value()) {
+    TORCH_CHECK(allowed->device() == logits.device() && allowed->scalar_type() == at::kInt && allowed->size(-1) == (V + 31) / 32 &&
+                    (allowed->stride(-1) == 1 || allowed->size(-1) == 1) &&
+                    (allowed->dim() == 1 || (allowed->dim() == 2 && allowed->size(0) == R)),
+                who, ": allowed must be int32 [(vocabulary + 31) / 32] or one such row per row of logits, on their device");
+    a.allowed = allowed->data_ptr<int>();
+    a.allowed_ld = allowed->dim() == 2 ? allowed->stride(0) : 0;
+  }
+  c10::DeviceGuard guard(logits.device());
+  Tensor o;
+  if (out.has_value()) {
+    o = *out;
+    TORCH_CHECK(o.device() == logits.device() && o.scalar_type() == logits.scalar_type() && o.sizes() == logits.sizes() &&
+                    (o.stride(1) == 1 || V == 1),
+                who, ": out must look like the logits, with unit inner stride");
+    at::assert_no_internal_overlap(o);
+    at::assert_no_partial_overlap(o, logits);   // in place is fine: every element is read and written by one thread
+  } else {
+    o = at::empty({R, V}, logits.options());
+  }
+  a.logits = logits.data_ptr();
+  a.out = o.data_ptr();
+  a.ld = logits.stride(0);
+  a.out_ld = o.stride(0);
+  a.R = (int)R;
+  a.V = (int)V;
+  dpa::penalize_logits(a, gemm_cus(), cur_stream());
+  return out.has_value() ? Tensor() : o;
+}
+
 TORCH_LIBRARY(dpa, m) {
   m.def("gemm_nt(Tensor a, Tensor b, Tensor? bias, int epi, Tensor? aux) -> (Tensor, Tensor?)");
   m.def("gemm_nt_supported(Tensor a, Tensor b, Tensor? bias, Tensor? aux) -> bool");
@@ -1345,6 +1616,14 @@ TORCH_LIBRARY(dpa, m) {
   m.def("decode_linear_supported(Tensor x, Tensor w, int act, bool has_ln) -> bool");
   m.def("gemm_nt_rope(Tensor a, Tensor b, Tensor? bias, Tensor rope_cos, Tensor rope_sin, int pos0, int seq_len, "
         "int rope_cols, int hs) -> Tensor");
+  m.def("paged_plan(Tensor q_lens, Tensor ctx_lens, Tensor(a!) table, Tensor free_pages, Tensor free_count, int page, "
+        "int tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("paged_append(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor k, Tensor v, Tensor slots) -> ()");
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor cu_q, Tensor kv_lens, float scale, "
+        "int window, int max_q, Tensor(a!)? out) -> Tensor");
+  m.def("penalize_logits(Tensor logits, Tensor? tokens, Tensor? prompt_lens, Tensor? total_lens, Tensor? repetition, "
+        "Tensor? presence, Tensor? frequency, float repetition_v, float presence_v, float frequency_v, Tensor? bias, "
+        "Tensor? allowed, Tensor(a!)? out) -> Tensor");
   m.def("rope_(Tensor(a!) x, Tensor cos_t, Tensor sin_t, int pos0, bool inverse) -> ()");
 }
 
@@ -1412,4 +1691,8 @@ TORCH_LIBRARY_IMPL(dpa, CUDA, m) {
   m.impl("attn_bwd", attn_bwd);
   m.impl("attn_decode", attn_decode);
   m.impl("rope_", rope_);
+  m.impl("paged_plan", paged_plan);
+  m.impl("paged_append", paged_append);
+  m.impl("paged_attention", paged_attention);
+  m.impl("penalize_logits", penalize_logits);
 }

@@ -298,4 +298,83 @@ void spin(int blocks, int usec, float* sink, hipStream_t st);
 void rope_inplace(void* x, long long bs, int ts, int B, int T_len, int nheads, int hs, const float* cos_t,
                   const float* sin_t, int pos0, bool inverse, bool is_bf16, hipStream_t st);
 
+// ---- Paged KV cache (ragged batches) -------------------------------------------------------
+// A pool of pages [P, page, nkv, width] holds the key / value rows of all requests; row j of request r lives in page
+// table[r, j / page] at row j % page. Lengths, tables and slots are int32 in device memory and read by the kernels only,
+// so every call can sit in a captured graph.
+struct FastDiv {   // division by a host-known divisor, see fast_div()
+  unsigned mul = 1;
+  int shift = 0;
+};
+inline FastDiv make_fast_div(int d) {
+  FastDiv f;
+  while ((1ll << f.shift) < d) ++f.shift;
+  f.mul = (unsigned)((((1ull << f.shift) - (unsigned long long)d) << 32) / (unsigned long long)d + 1);
+  return f;
+}
+enum { kTypeBf16 = 0, kTypeHalf = 1, kTypeFloat = 2 };
+
+// Pages for the new tokens of R requests and where their rows go (csrc/paged_plan.hip states the formulas).
+// page >= 1, 0 <= tokens < 2^30; every array int32. free_left: {pages left, pages missing}.
+struct PagedPlanArgs {
+  const int *q_lens, *ctx_lens;
+  int* table;
+  long long table_ld;
+  const int *free_pages, *free_count;
+  int free_cap;
+  int R, M, page, tokens;
+  FastDiv by_page;
+  int *cu_q, *kv_lens, *positions, *slots, *free_left;
+};
+void paged_plan(const PagedPlanArgs& a, hipStream_t st);
+
+// Rows k[i], v[i] ([nkv, dk] / [nkv, dv], strides in elements, unit inner stride) -> row slots[i] of the pools; slots
+// outside [0, pages * page) are skipped. elem: bytes per element (2 or 4).
+struct PagedAppendArgs {
+  void *k_pages, *v_pages;
+  const void *k, *v;
+  const int* slots;
+  long long kp_ps, kp_rs, kp_hs, vp_ps, vp_rs, vp_hs;   // page / row / head strides of the pools
+  long long k_ts, k_hs, v_ts, v_hs;                     // token / head strides of the new rows
+  int N, nkv, dk, dv, pages, page, elem;
+  FastDiv by_page;
+};
+void paged_append(const PagedAppendArgs& a, hipStream_t st);
+
+// Causal attention of the newest tokens of every request over its pages (csrc/paged_attn.hip).
+struct PagedAttnArgs {
+  const void *q, *k, *v;
+  void* o;
+  const int *table, *cu_q, *kv_lens;
+  long long table_ld;
+  long long q_ts, q_hs, o_ts, o_hs;
+  long long k_ps, k_rs, k_hs, v_ps, v_rs, v_hs;
+  int N, R, M, nh, nkv, width, pages, page;
+  FastDiv by_page;
+  float scale;
+  int window;        // 0: none
+  int max_q;         // no request has more new tokens (rows past it are left alone)
+  int type;          // kTypeBf16 / kTypeHalf / kTypeFloat
+  bool zero_rest;    // rows outside every sequence: true = zeroed, false = left as they are
+};
+void paged_attn(const PagedAttnArgs& a, hipStream_t st);
+
+// ---- Logit penalties (csrc/penalties.hip) -----------------------------------------------------
+struct PenaltyArgs {
+  const void* logits;
+  void* out;
+  const void* tokens;          // [R, L] int64 or int32, or nullptr
+  bool tokens64;
+  const int *prompt_lens, *total_lens;          // entry r * stride (stride 0: one value for all rows), or nullptr
+  int prompt_stride, total_stride;
+  const float *repetition, *presence, *frequency;   // same, fp32; nullptr: the value below
+  int repetition_stride, presence_stride, frequency_stride;
+  float repetition_v, presence_v, frequency_v;
+  const float* bias;           // [R, V] row stride bias_ld (0: shared), or nullptr
+  const int* allowed;          // bit v % 32 of word v / 32, row stride allowed_ld (0: shared), or nullptr
+  long long ld, out_ld, tokens_ld, bias_ld, allowed_ld;
+  int R, V, L, type;
+};
+void penalize_logits(const PenaltyArgs& a, int num_cus, hipStream_t st);
+
 }  // namespace dpa

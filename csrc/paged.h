@@ -1,0 +1,22 @@
+// Shared pieces of the paged-cache kernels (csrc/paged_plan.hip, paged_append.hip, paged_attn*.hip).
+#pragma once
+#include "common.h"
+#include "kernels.h"
+
+namespace dpa {
+
+typedef _Float16 half_t;
+
+template <> struct Cvt<half_t> {
+  static __device__ __forceinline__ float ld(const half_t* p) { return (float)*p; }
+  static __device__ __forceinline__ void st(half_t* p, float v) { *p = (half_t)v; }   // round to nearest even
+};
+
+// n / d for 0 <= n < 2^31 and a divisor known on the host: q = (n + hi32(n * mul)) >> shift with
+// shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1 (the round-up method of division by invariant integers;
+// the sum stays below 2^32 because hi32(n * mul) <= n).
+__device__ __forceinline__ int fast_div(int n, const FastDiv& f) {
+  return (int)((__umulhi((unsigned)n, f.mul) + (unsigned)n) >> f.shift);
+}
+
+}  // namespace dpa

@@ -16,8 +16,9 @@ from .moe import (expert_counts, gather_combine, grouped_experts, grouped_expert
 from .moe import plan as moe_plan
 from .norm import add_layer_norm, layer_norm, layer_norm_keep
 from .optim import adamw_step, sumsq
+from .paged import PagedPlan, paged_append, paged_attention, paged_attention_eager, paged_plan
 from .rope import apply_rope, rope_inplace_, rope_tables, rope_qkv_
-from .sampling import sample_eager, sample_fused, sample_step, sample_step_supported
+from .sampling import penalize_logits, penalize_logits_eager, sample_eager, sample_fused, sample_step, sample_step_supported
 
 __all__ = [
     "gelu", "swiglu", "get_activation", "cached_attention", "causal_attention", "causal_attention_eager", "causal_self_attention_qkv", "dropout_keep_mask", "kv_append",
@@ -26,4 +27,5 @@ __all__ = [
     "IGNORE_INDEX", "layer_norm", "add_layer_norm", "layer_norm_keep", "adamw_step", "sumsq", "apply_rope", "rope_inplace_",
     "rope_tables", "linear", "mlp_gelu", "mlp_gelu_supported", "mlp_swiglu", "mlp_swiglu_supported", "bump_weights_epoch", "transposed_weight", "weight_grad", "wgrad_supported", "grouped_experts", "grouped_experts_eager",
     "grouped_supported", "expert_counts", "sample_eager", "sample_fused", "sample_step", "sample_step_supported", "topk_gate", "moe_plan", "plan_dense", "scatter_rows", "gather_combine",
+    "PagedPlan", "paged_plan", "paged_append", "paged_attention", "paged_attention_eager", "penalize_logits", "penalize_logits_eager",
 ]

@@ -53,3 +53,86 @@ def sample_fused(logits: torch.Tensor, temperature: float = 1.0, topk: int | Non
     if seed is None:
         seed = torch.randint(-(1 << 62), 1 << 62, (1,), dtype=torch.int64, device=logits.device)
     return ops().sample_topk(logits, float(temperature), int(topk or 0), seed)
+
+
+def _row_value(x, logits: torch.Tensor):
+    """(device vector or None, host value) of a penalty given as a number or an fp32 tensor (one value, or one per row)."""
+    return (x, 0.0) if isinstance(x, torch.Tensor) else (None, float(x))
+
+
+def penalize_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                    total_lens: torch.Tensor | None = None, repetition=1.0, presence=0.0, frequency=0.0,
+                    bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits ``[R, V]`` (bf16, fp16, fp32) with penalties for repeated tokens, biases and a grammar mask applied, for the
+    sampler that follows. ``tokens [R, L]`` (int64 or int32) is the rows' history, of which the first ``total_lens``
+    entries count (default: all) and the first ``prompt_lens`` are the prompt (default: none); ids outside the
+    vocabulary are ignored. In fp32, rounded once:
+
+    * ``repetition``: the logit of every token in the history is divided by it where positive, multiplied elsewhere;
+    * ``presence`` and ``frequency``: a token generated n > 0 times loses ``presence + n * frequency``;
+    * ``bias`` (fp32 ``[V]`` or ``[R, V]``) is added;
+    * ``allowed`` (int32 ``[ceil(V / 32)]`` or one such row per row of logits): tokens whose bit ``v % 32`` of word ``v // 32``
+      is clear become -inf, whatever their logit was. A row that allows nothing is -inf throughout.
+
+    The penalties are numbers or fp32 tensors with one value or one per row, lengths int32 tensors likewise; they are
+    read by the kernel, so a captured step sees what a replay's buffers hold. ``out`` may be ``logits`` itself."""
+    if use_hip(logits):
+        rep, rep_v = _row_value(repetition, logits)
+        pres, pres_v = _row_value(presence, logits)
+        freq, freq_v = _row_value(frequency, logits)
+        y = ops().penalize_logits(logits, tokens, prompt_lens, total_lens, rep, pres, freq, rep_v, pres_v, freq_v, bias, allowed,
+                                  out)
+        return y if out is None else out
+    return penalize_logits_eager(logits, tokens, prompt_lens, total_lens, repetition, presence, frequency, bias, allowed, out)
+
+
+def penalize_logits_eager(logits, tokens=None, prompt_lens=None, total_lens=None, repetition=1.0, presence=0.0, frequency=0.0,
+                          bias=None, allowed=None, out=None) -> torch.Tensor:
+    """The same computation with stock ops (CPU; fp64 logits for checks)."""
+    def check(ok, message):
+        if not ok:
+            raise RuntimeError("penalize_logits: " + message)
+
+    check(logits.dim() == 2, "logits must be [rows, vocabulary]")
+    R, V = logits.shape
+    dev = logits.device
+    real = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    x = logits.to(real)
+
+    def column(value, name, dtype):
+        if not isinstance(value, torch.Tensor):
+            return torch.full((1, 1), value, dtype=real, device=dev)
+        check(value.dtype == dtype and value.dim() == 1 and value.numel() in (1, R), f"{name} must be one value or one per row")
+        return value.view(-1, 1)
+
+    if tokens is not None:
+        check(tokens.dim() == 2 and tokens.shape[0] == R and tokens.dtype in (torch.int64, torch.int32),
+              "tokens must be int64 or int32 [rows, history]")
+        L = tokens.shape[1]
+        j = torch.arange(L, device=dev)[None, :]
+        total = column(L if total_lens is None else total_lens, "total_lens", torch.int32)
+        prompt = column(0 if prompt_lens is None else prompt_lens, "prompt_lens", torch.int32)
+        live = (j < total) & (tokens >= 0) & (tokens < V)
+        at = torch.where(live, tokens.long(), torch.zeros_like(tokens, dtype=torch.int64))
+        seen = torch.zeros(R, V, dtype=torch.int32, device=dev).scatter_add_(1, at, live.int()) > 0
+        count = torch.zeros(R, V, dtype=torch.int32, device=dev).scatter_add_(1, at, (live & (j >= prompt)).int())
+        rep = column(repetition, "repetition", torch.float32).to(real)
+        x = torch.where(seen, torch.where(x > 0, x / rep, x * rep), x)
+        lost = column(frequency, "frequency", torch.float32).to(real) * count.to(real) + \
+            column(presence, "presence", torch.float32).to(real)
+        x = torch.where(count > 0, x - lost, x)
+    if bias is not None:
+        check(bias.dtype == torch.float32 and bias.shape in ((V,), (R, V)), "bias must be fp32 [vocabulary] or [rows, vocabulary]")
+        x = x + bias.to(real)
+    if allowed is not None:
+        words = (V + 31) // 32
+        check(allowed.dtype == torch.int32 and allowed.shape in ((words,), (R, words)),
+              "allowed must be int32 [(vocabulary + 31) / 32] or one such row per row of logits")
+        v = torch.arange(V, device=dev)
+        bit = (allowed[..., v // 32] >> (v % 32).to(torch.int32)) & 1
+        x = x.masked_fill(bit == 0, float("-inf"))
+    if out is None:
+        return x.to(logits.dtype)
+    check(out.shape == logits.shape and out.dtype == logits.dtype, "out must look like the logits")
+    return out.copy_(x)

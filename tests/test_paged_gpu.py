@@ -1,0 +1,566 @@
+"""Paged cache operators and logit penalties on the GPU against plain forms in 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from distributed_pytorch_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+# ---- planning -------------------------------------------------------------------------------------
+def plan_case(R, N, page, top_ctx, seed, spare=3, single=False):
+    """Random lengths that sum to N, a table filled for the cached rows, a shuffled free list."""
+    rng = random.Random(seed)
+    if single:
+        q = [1] * N + [0] * (R - N)
+    else:
+        cuts = sorted(rng.randint(0, N) for _ in range(R - 1))
+        q = [b - a for a, b in zip([0] + cuts, cuts + [N])]
+    c = [rng.choice([0, rng.randint(0, top_ctx), page * rng.randint(0, top_ctx // page)]) for _ in range(R)]
+    pages = [-(-n // page) for n in c]
+    cols = max(-(-(a + b) // page) for a, b in zip(q, c)) + 1
+    ids = list(range(sum(pages) + N + spare))
+    rng.shuffle(ids)
+    table = torch.full((R, cols), -1, dtype=torch.int32)
+    for r, n in enumerate(pages):
+        table[r, :n] = torch.tensor([ids.pop() for _ in range(n)], dtype=torch.int32)
+    free = torch.tensor(ids, dtype=torch.int32)
+    return torch.tensor(q, dtype=torch.int32), torch.tensor(c, dtype=torch.int32), table, free
+
+
+@pytest.mark.parametrize("R,N,page,top,pad,single", [
+    (1, 1, 16, 100, 0, False), (1, 0, 16, 100, 3, False), (7, 4099, 16, 300, 5, False), (64, 64, 16, 1000, 0, True), (200, 1023, 1, 30, 2, False),
+    (1025, 1024, 24, 200, 0, True), (2050, 5000, 32, 60, 100, False), (3, 2048, 128, 500, 0, False)])
+def test_plan_matches_the_host_form(R, N, page, top, pad, single):
+    q, c, table, free = plan_case(R, N, page, top, seed=R + N, single=single)
+    count = torch.tensor([free.numel() - 1], dtype=torch.int32)
+    want_table = table.clone()
+    want = ops.paged_plan(q, c, want_table, free, count, page, N + pad)
+    got_table = table.to(DEV)
+    args = (q.to(DEV), c.to(DEV), got_table, free.to(DEV), count.to(DEV), page, N + pad)
+    for _ in range(2):      # the inputs are not changed: a second call gives the same
+        got = ops.paged_plan(*args)
+        assert torch.equal(got_table.cpu(), want_table)
+        for name, a, b in zip(want._fields, got, want):
+            assert torch.equal(a.cpu(), b), name
+
+
+@pytest.mark.parametrize("count,cols,rows", [(0, 4, 40), (3, 4, 40), (40, 1, 40), (40, 4, 17), (-5, 4, 40), (1000, 4, 40), (40, 0, 40)])
+def test_plan_short_of_pages_columns_and_rows(count, cols, rows):
+    q, c = torch.tensor([5, -3, 9, 20, 6], dtype=torch.int32), torch.tensor([3, 0, 8, -1, 7], dtype=torch.int32)
+    table = torch.arange(100, 100 + 5 * cols, dtype=torch.int32).view(5, cols)
+    free = torch.arange(40, dtype=torch.int32).flip(0)
+    want_table, got_table = table.clone(), torch.full((5, cols + 3), -9, dtype=torch.int32, device=DEV)
+    view = got_table[:, :cols]
+    view.copy_(table)
+    want = ops.paged_plan(q, c, want_table, free, torch.tensor([count], dtype=torch.int32), 8, rows)
+    got = ops.paged_plan(q.to(DEV), c.to(DEV), view, free.to(DEV), i32(count), 8, rows)
+    assert torch.equal(view.cpu(), want_table) and (got_table[:, cols:] == -9).all()
+    for name, a, b in zip(want._fields, got, want):
+        assert torch.equal(a.cpu(), b), name
+
+
+# ---- append ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("N,nkv,dk,dv,page", [(1, 1, 64, 64, 16), (65, 12, 64, 64, 16), (300, 8, 128, 64, 24), (77, 3, 20, 7, 1), (130, 2, 96, 96, 5)])
+def test_append_writes_the_rows_and_nothing_else(dtype, N, nkv, dk, dv, page):
+    g = torch.Generator(device=DEV).manual_seed(N)
+    pages = -(-N // page) + 4
+    fused = torch.randn(N, nkv * (dk + dv) + 8, device=DEV, generator=g).to(dtype)
+    k = fused[:, :nkv * dk].view(N, nkv, dk)
+    v = fused[:, nkv * dk: nkv * (dk + dv)].view(N, nkv, dv)
+    slots = torch.randperm(pages * page, device=DEV, generator=g)[:N].int()
+    if N > 10:
+        slots[3], slots[7], slots[9] = -1, pages * page, 2 ** 31 - 1
+    kp = torch.full((pages, page, nkv, dk), 3.0, dtype=dtype, device=DEV)
+    vp = torch.full((pages, nkv, page, dv), 5.0, dtype=dtype, device=DEV).transpose(1, 2)      # heads outside the rows
+    want_k, want_v = kp.clone(), vp.clone()
+    keep = (slots >= 0) & (slots < pages * page)
+    at = slots[keep].long()
+    want_k[at // page, at % page] = k[keep]
+    want_v[at // page, at % page] = v[keep]
+    ops.paged_append(kp, vp, k, v, slots)
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+# ---- attention --------------------------------------------------------------------------------------
+def pool(kv, page, nkv, width, dtype, g, spare=2, columns=0):
+    """Pages of the requests scattered over a pool; rows no request owns hold NaN, free columns of the table rubbish."""
+    counts = [-(-n // page) for n in kv]
+    ids = torch.randperm(sum(counts) + spare, generator=torch.Generator().manual_seed(sum(kv))).int()
+    table = torch.full((len(kv), max(counts + [1]) + columns), -7, dtype=torch.int32)
+    k = torch.full((sum(counts) + spare, page, nkv, width), math.nan, device=DEV)
+    v = k.clone()
+    at = 0
+    for r, n in enumerate(kv):
+        mine = ids[at:at + counts[r]]
+        at += counts[r]
+        table[r, :counts[r]] = mine
+        for j, p in enumerate(mine.tolist()):
+            m = min(page, n - j * page)
+            k[p, :m] = torch.randn(m, nkv, width, device=DEV, generator=g)
+            v[p, :m] = torch.randn(m, nkv, width, device=DEV, generator=g)
+    return k.to(dtype), v.to(dtype), table.to(DEV)
+
+
+def bound(q, k, v, table, cu, kv, scale, window, n_max):
+    """The exact result in 64 bits, and the error that the formula's roundings allow, element by element. With u the
+    half step of the type: each probability may be rounded to the type before the product (u), the result is (u);
+    a score is an fp32 sum of width products (width + 4 roundings of its terms' size, at most |q| |k| scale) and moves
+    numerator and denominator; the sums over n keys are fp32. All relative to sum w |v|, which bounds |o|."""
+    exact = ops.paged_attention_eager(q.double(), k.double(), v.double(), table, cu, kv, scale, window)
+    size = ops.paged_attention_eager(q.double(), k.double(), v.double().abs(), table, cu, kv, scale, window)
+    u = half_step(q.dtype)
+    kn = torch.nan_to_num(k.float(), 0.0, 0.0, 0.0).norm(dim=-1).max().item()
+    top = scale * q.float().norm(dim=-1).max().item() * kn
+    f = 2.0 ** -24
+    score = (q.shape[-1] + 4) * f * top + 4 * f * (1 + top)       # and the exponential with its argument
+    return exact, size * (2 * u + 2 * score + (n_max + 4) * f) * 1.01 + torch.finfo(q.dtype).tiny
+
+
+def check_attention(qn, ctx, nh, nkv, width, page, dtype, window=None, max_q=None, pad=0, gain=1.0):
+    g = torch.Generator(device=DEV).manual_seed(sum(qn) * 31 + sum(ctx))
+    kv = [a + b for a, b in zip(qn, ctx)]
+    k, v, table = pool(kv, page, nkv, width, dtype, g, columns=2)
+    cu = [0]
+    for n in qn:
+        cu.append(cu[-1] + n)
+    q = (torch.randn(cu[-1] + pad, nh, width, device=DEV, generator=g) * gain).to(dtype)
+    scale = 1 / math.sqrt(width)
+    cu, kv = i32(*cu), i32(*kv)
+    o = ops.paged_attention(q, k, v, table, cu, kv, window=window, max_q=max_q)
+    want, tol = bound(q, k, v, table, cu, kv, scale, window, max([1] + kv.tolist()))
+    err = (o.double() - want).abs()
+    assert torch.isfinite(o).all()
+    assert (err <= tol).all(), f"worst {(err / tol).max().item():.3f} of the bound, at {(err - tol).argmax().item()}"
+    return q, k, v, table, cu, kv, o
+
+
+SHAPES = [  # heads, kv heads, width
+    (12, 12, 64), (8, 2, 128), (8, 1, 64), (6, 2, 96), (4, 4, 32), (9, 3, 80), (16, 2, 128), (40, 1, 64)]
+
+
+@pytest.mark.parametrize("nh,nkv,width", SHAPES)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_one_token_per_request(nh, nkv, width, dtype):
+    check_attention([1] * 9, [0, 1, 15, 16, 31, 63, 64, 300, 1111], nh, nkv, width, 16, dtype, max_q=1)
+
+
+@pytest.mark.parametrize("nh,nkv,width", SHAPES)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_chunks_next_to_single_tokens(nh, nkv, width, dtype):
+    check_attention([1, 129, 0, 1, 200, 5, 64], [500, 0, 0, 77, 333, 60, 64], nh, nkv, width, 24, dtype, pad=3)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 16, 64, 100, 256])
+def test_attention_page_sizes(page):
+    check_attention([1, 70, 3], [400, 130, 0], 8, 2, 64, page, BF)
+    check_attention([1, 70, 3], [400, 130, 0], 4, 2, 128, page, BF)
+
+
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 5000])
+@pytest.mark.parametrize("width", [64, 128])
+def test_attention_window(window, width):
+    check_attention([1, 150, 1, 33], [900, 200, 10, 0], 4, 2, width, 16, BF, window=window)
+    check_attention([1, 1, 2], [4000, 100, 900], 8, 2, width, 16, BF, window=window, max_q=2)
+
+
+@pytest.mark.parametrize("qn,ctx", [([1], [20000]), ([1, 1], [30000, 5]), ([4], [9000]), ([300], [6000]), ([1] * 70, list(range(0, 7000, 100)))])
+@pytest.mark.parametrize("width", [64, 128])
+def test_attention_long_contexts(qn, ctx, width):
+    check_attention(qn, ctx, 8, 2, width, 16, BF)
+
+
+@pytest.mark.parametrize("dtype,width", [(FP, 64), (FP, 100), (BF, 20), (HF, 7), (BF, 200), (BF, 256), (FP, 1)])
+def test_attention_other_types_and_widths(dtype, width):
+    check_attention([1, 40, 0, 2], [100, 33, 0, 0], 4, 2, width, 16, dtype, pad=1)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("gain", [20.0, 200.0])
+def test_attention_large_scores(dtype, gain):
+    """Scores of hundreds: weights collapse on single keys, and a running maximum moves by more than any exponent range."""
+    check_attention([1, 90], [700, 200], 4, 2, 64, 16, dtype, gain=gain)
+    check_attention([1, 90], [700, 200], 4, 2, 128, 16, dtype, gain=gain)
+
+
+def test_attention_rising_and_falling_scores():
+    """The maximum arrives last, or first, by a margin that drowns every other key."""
+    for order in (1, -1):
+        g = torch.Generator(device=DEV).manual_seed(5)
+        k, v, table = pool([600], 16, 1, 64, BF, g)
+        ramp = torch.linspace(-30, 30, 600, device=DEV) * order
+        rows = (table[0, :38].long()[:, None] * 16 + torch.arange(16, device=DEV)).flatten()[:600]
+        k.view(-1, 64)[rows] = (ramp[:, None] * torch.ones(64, device=DEV) / 8).to(BF)
+        q = torch.ones(130, 2, 64, dtype=BF, device=DEV)
+        for n in (1, 130):
+            cu, kv = i32(0, n), i32(600)
+            o = ops.paged_attention(q[:n], k, v, table, cu, kv)
+            want, tol = bound(q[:n], k, v, table, cu, kv, 1 / 8, None, 600)
+            assert ((o.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 60, 200])
+def test_attention_rows_before_the_first_key_are_zero(n):
+    g = torch.Generator(device=DEV).manual_seed(n)
+    k, v, table = pool([n // 3, 0], 16, 2, 64, BF, g)
+    q = torch.randn(2 * n, 4, 64, device=DEV, generator=g).to(BF)
+    cu, kv = i32(0, n, 2 * n), i32(n // 3, 0)
+    o = ops.paged_attention(q, k, v, table, cu, kv)
+    assert (o[: n - n // 3] == 0).all() and (o[n:] == 0).all()
+    want, tol = bound(q, k, v, table, cu, kv, 1 / 8, None, n)
+    assert ((o.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 100])
+@pytest.mark.parametrize("width", [64, 128])
+def test_attention_missing_pages_are_left_out(n, width):
+    g = torch.Generator(device=DEV).manual_seed(n)
+    k, v, table = pool([400, 300], 16, 2, width, BF, g)
+    q = torch.randn(2 * n, 4, width, device=DEV, generator=g).to(BF)
+    cu, kv = i32(0, n, 2 * n), i32(400, 300)
+    table[0, 0], table[0, 7], table[0, 24], table[1, 3] = -1, k.shape[0], 2 ** 31 - 1, -2 ** 31
+    o = ops.paged_attention(q, k, v, table, cu, kv)
+    want, tol = bound(q, k, v, table, cu, kv, 1 / math.sqrt(width), None, 400)
+    assert ((o.double() - want).abs() <= tol).all()
+    table.fill_(-1)
+    assert (ops.paged_attention(q, k, v, table, cu, kv) == 0).all()
+
+
+@pytest.mark.parametrize("n,window", [(2, None), (70, None), (200, None), (200, 50), (3, 20)])
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_values_in_masked_places_stay_there(n, window, width, bad):
+    """A key or value that is not finite reaches the rows that see it and no others."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    L = n + 40
+    k, v, table = pool([L], 16, 2, width, BF, g)
+    q = torch.randn(n, 4, width, device=DEV, generator=g).to(BF)
+    cu, kv = i32(0, n), i32(L)
+    at = L - 1 - n // 2              # the position of the row in the middle
+    slot = int(table[0, at // 16]) * 16 + at % 16
+    clean = ops.paged_attention(q, k, v, table, cu, kv, window=window)
+    v.view(-1, 2, width)[slot, :, 3] = bad
+    o = ops.paged_attention(q, k, v, table, cu, kv, window=window)
+    pos = torch.arange(L - n, L, device=DEV)
+    sees = pos >= at
+    if window:
+        sees &= pos < at + window
+    assert torch.equal(o[~sees], clean[~sees]) and not torch.isfinite(o[sees][:, :, 3]).any()
+    rest = [d for d in range(width) if d != 3]
+    assert torch.equal(o[..., rest], clean[..., rest])
+    v.view(-1, 2, width)[slot, :, 3] = 0
+    k.view(-1, 2, width)[slot] = math.nan
+    o = ops.paged_attention(q, k, v, table, cu, kv, window=window)
+    assert torch.isfinite(o[~sees]).all() and torch.isnan(o[sees]).all()
+
+
+def test_attention_strided_operands_and_out():
+    g = torch.Generator(device=DEV).manual_seed(1)
+    N, nh, nkv, d = 75, 8, 2, 64
+    qn, kv = [70, 5], [200, 90]
+    k, v, table = pool(kv, 16, nkv, d, BF, g)
+    fused = torch.randn(N, (nh + 2 * nkv) * d, device=DEV, generator=g).to(BF)
+    q = fused[:, : nh * d].view(N, nh, d)
+    cu, lens = i32(0, 70, 75), i32(*kv)
+    plain = ops.paged_attention(q.contiguous(), k, v, table, cu, lens)
+    out = torch.full((N, 2 * nh, d), 9.0, dtype=BF, device=DEV)
+    ops.paged_attention(q, k, v, table, cu, lens, out=out[:, ::2])
+    assert torch.equal(out[:, ::2], plain) and (out[:, 1::2] == 9.0).all()
+    heads_first = k.transpose(1, 2).contiguous().transpose(1, 2)
+    both = torch.stack([k, v], 1)      # keys and values of a page next to each other
+    wide_table = torch.full((4, 40), -3, dtype=torch.int32, device=DEV)
+    wide_table[::2, : table.shape[1]] = table
+    for kk, vv in ((heads_first, v), (both[:, 0], both[:, 1])):
+        assert torch.equal(ops.paged_attention(q, kk, vv, table, cu, lens), plain)
+    assert torch.equal(ops.paged_attention(q, k, v, wide_table[::2], cu, lens), plain)
+    # rows that no 16-byte access can reach
+    odd = torch.empty(k.numel() + 1, dtype=BF, device=DEV)[1:].view_as(k).copy_(k)
+    want, tol = bound(q, k, v, table, cu, lens, 1 / 8, None, 200)
+    assert ((ops.paged_attention(q, odd, v, table, cu, lens).double() - want).abs() <= tol).all()
+
+
+def test_attention_leaves_rows_outside_the_requests():
+    g = torch.Generator(device=DEV).manual_seed(2)
+    k, v, table = pool([50], 16, 1, 64, BF, g)
+    q = torch.randn(20, 2, 64, device=DEV, generator=g).to(BF)
+    for n in (1, 12):
+        out = torch.full_like(q, 4.0)
+        ops.paged_attention(q, k, v, table, i32(3, 3 + n), i32(50), out=out)
+        assert (out[:3] == 4).all() and (out[3 + n:] == 4).all() and not (out[3:3 + n] == 4).all()
+        fresh = ops.paged_attention(q, k, v, table, i32(3, 3 + n), i32(50))
+        assert (fresh[:3] == 0).all() and (fresh[3 + n:] == 0).all() and torch.equal(fresh[3:3 + n], out[3:3 + n])
+    none = torch.zeros(0, 3, dtype=torch.int32, device=DEV)
+    assert (ops.paged_attention(q, k, v, none, i32(0), i32()) == 0).all()
+    assert ops.paged_attention(q[:0], k, v, table, i32(0, 0), i32(50)).shape == (0, 2, 64)
+
+
+def test_attention_lengths_that_contradict_the_buffers():
+    """Lengths past the table, past the batch or below zero stay inside the buffers (results of such rows are unspecified)."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    k, v, table = pool([60, 60], 16, 1, 64, BF, g)
+    q = torch.randn(40, 2, 64, device=DEV, generator=g).to(BF)
+    for cu, kv in (((0, 20, 4000), (60, 60)), ((0, 20, 40), (10 ** 9, 2 ** 31 - 1)), ((-50, 20, 40), (60, -5)), ((0, 40, 20), (60, 60)),
+                   ((5, 0, 2 ** 31 - 1), (-2 ** 31, 60))):
+        out = ops.paged_attention(q, k, v, table, i32(*cu), i32(*kv))
+        torch.cuda.synchronize()
+        assert out.shape == q.shape
+
+
+def test_attention_offsets_past_32_bits():
+    """Pools of more than 2^32 bytes and 2^31 elements, used at both ends."""
+    P, page, nkv, d = 140000, 16, 8, 128
+    k = torch.empty(P, page, nkv, d, dtype=BF, device=DEV)
+    v = torch.empty(P, page, nkv, d, dtype=BF, device=DEV)
+    assert k.numel() > 2 ** 31
+    g = torch.Generator(device=DEV).manual_seed(3)
+    ids = [P - 1, 0, P - 2, 131072, 70000, 1, P - 3]
+    small = torch.randn(2, len(ids), page, nkv, d, device=DEV, generator=g).to(BF)
+    table = i32(*ids).view(1, -1)
+    L = page * len(ids)
+    slots = (table.view(-1, 1) * page + torch.arange(page, device=DEV, dtype=torch.int32)).flatten().contiguous()
+    ops.paged_append(k, v, small[0].view(L, nkv, d), small[1].view(L, nkv, d), slots)
+    assert torch.equal(k[ids], small[0]) and torch.equal(v[ids], small[1])
+    for n in (1, 100):
+        q = torch.randn(n, 16, d, device=DEV, generator=g).to(BF)
+        o = ops.paged_attention(q, k, v, table, i32(0, n), i32(L))
+        near = torch.arange(len(ids), device=DEV, dtype=torch.int32).view(1, -1)
+        assert torch.equal(o, ops.paged_attention(q, small[0], small[1], near, i32(0, n), i32(L)))
+
+
+# ---- penalties -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("R,V,L,ids", [(1, 50304, 300, torch.int64), (3, 50257, 2000, torch.int32), (9, 65, 40, torch.int64), (2, 1, 3, torch.int64),
+                                       (5, 8193, 70000, torch.int32), (4, 200003, 500, torch.int64), (6, 1000, 0, torch.int64)])
+def test_penalties(dtype, R, V, L, ids):
+    g = torch.Generator(device=DEV).manual_seed(V)
+    logits = (torch.randn(R, V, device=DEV, generator=g) * 4).to(dtype)
+    tokens = ((torch.rand(R, L, device=DEV, generator=g) ** 4) * (V + 3)).to(ids) - 1       # a few outside the vocabulary
+    total = torch.randint(-2, L + 3, (R,), device=DEV, generator=g).int()
+    prompt = torch.randint(-2, L + 3, (R,), device=DEV, generator=g).int()
+    rep = torch.rand(R, device=DEV, generator=g) + 0.7
+    freq, pres = torch.rand(R, device=DEV, generator=g) - 0.2, torch.rand(1, device=DEV, generator=g)
+    bias = torch.randn(R, V, device=DEV, generator=g)
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (R, (V + 31) // 32), device=DEV, generator=g).int()
+    if R > 2:
+        allowed[2] = 0
+    u = half_step(dtype)
+    for b, m in ((None, None), (bias, allowed), (bias[0].contiguous(), allowed[0].contiguous()), (None, allowed)):
+        kw = dict(repetition=rep, presence=pres, frequency=freq, bias=b, allowed=m)
+        got = ops.penalize_logits(logits, tokens, prompt, total, **kw)
+        want = ops.penalize_logits_eager(logits.double(), tokens, prompt, total, **kw)
+        assert got.dtype == dtype and torch.equal(torch.isinf(got), torch.isinf(want))
+        fin = torch.isfinite(want)
+        # one rounding to the type; before it five fp32 operations on terms no larger than the sum below
+        size = logits.double().abs() * 1.7 / 0.7 + (L + 1.0) * 2 + (0 if b is None else b.double().abs())
+        hits = want.abs() * u + 6 * size * 2.0 ** -24 + torch.finfo(dtype).tiny
+        assert ((got.double() - want).abs()[fin] <= hits[fin]).all()
+        again = logits.clone()
+        assert ops.penalize_logits(again, tokens, prompt, total, out=again, **kw) is again
+        assert torch.equal(again, got)
+
+
+def test_penalties_strides_defaults_and_what_is_masked():
+    g = torch.Generator(device=DEV).manual_seed(0)
+    big = torch.randn(4, 1003, device=DEV, generator=g).to(BF)
+    view = big[:, 3:]
+    tokens = torch.randint(0, 1000, (4, 31), device=DEV, generator=g)
+    assert torch.equal(ops.penalize_logits(view), view)
+    got = ops.penalize_logits(view, tokens[:, 1:], repetition=1.5, frequency=0.25)
+    want = ops.penalize_logits(view.contiguous(), tokens[:, 1:].contiguous(), repetition=1.5, frequency=0.25)
+    assert torch.equal(got, want)
+    x = view.clone()
+    x[:, 7], x[:, 8], x[:, 9] = math.nan, math.inf, -math.inf
+    allowed = torch.full((32,), -1, dtype=torch.int32, device=DEV)
+    allowed[0] = ~(1 << 7 | 1 << 8)
+    y = ops.penalize_logits(x, allowed=allowed)
+    assert (y[:, 7:10] == -math.inf).all()
+    keep = [i for i in range(1000) if i not in (7, 8, 9)]
+    assert torch.equal(y[:, keep], x[:, keep])
+
+
+# ---- a run of them together, streams, graphs, refusals ----------------------------------------------------
+def test_steps_of_a_ragged_batch_match_one_pass():
+    """Three requests worked off in uneven chunks over shared pages give what one pass over each gives."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    nh, nkv, d, page, lens = 8, 2, 64, 16, [300, 41, 90]
+    qs = [torch.randn(n, nh, d, device=DEV, generator=g).to(BF) for n in lens]
+    ks = [torch.randn(n, nkv, d, device=DEV, generator=g).to(BF) for n in lens]
+    vs = [torch.randn(n, nkv, d, device=DEV, generator=g).to(BF) for n in lens]
+    P = sum(-(-n // page) for n in lens)
+    kp = torch.full((P, page, nkv, d), math.nan, dtype=BF, device=DEV)
+    vp = kp.clone()
+    table = torch.full((3, 20), -1, dtype=torch.int32, device=DEV)
+    free, left = torch.randperm(P, device=DEV, generator=g).int(), i32(P)
+    ctx = i32(0, 0, 0)
+    done, outs = [0, 0, 0], [[], [], []]
+    for step in ([100, 41, 1], [1, 0, 64], [130, 0, 1], [69, 0, 24]):
+        rows = [slice(done[r], done[r] + n) for r, n in enumerate(step)]
+        pad = torch.zeros(7, nh, d, dtype=BF, device=DEV)
+        q = torch.cat([qs[r][s] for r, s in enumerate(rows)] + [pad])
+        k = torch.cat([ks[r][s] for r, s in enumerate(rows)] + [pad[:, :nkv]])
+        v = torch.cat([vs[r][s] for r, s in enumerate(rows)] + [pad[:, :nkv]])
+        plan = ops.paged_plan(i32(*step), ctx, table, free, left, page, q.shape[0])
+        ops.paged_append(kp, vp, k, v, plan.slots)
+        o = ops.paged_attention(q, kp, vp, table, plan.cu_q, plan.kv_lens)
+        assert (o[sum(step):] == 0).all()
+        ctx, left = plan.kv_lens, plan.free_left
+        at = 0
+        for r, n in enumerate(step):
+            outs[r].append(o[at:at + n])
+            at += n
+            done[r] += n
+    assert done == lens and left.tolist() == [0, 0] and sorted(table[table >= 0].tolist()) == list(range(P))
+    for r, n in enumerate(lens):
+        mine = i32(0).view(1, 1)
+        want, tol = bound(qs[r], ks[r][None], vs[r][None], mine, i32(0, n), i32(n), 1 / 8, None, n)
+        assert ((torch.cat(outs[r]).double() - want).abs() <= tol).all()
+
+
+def test_captured_steps_follow_their_buffers():
+    """One captured decode step (plan, append, attention, penalties) replayed over growing requests, with eager work
+    between the replays; two graphs over the same pool."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    R, nh, nkv, d, page, V = 5, 4, 2, 64, 16, 1000
+    P = 60
+    start = [0, 15, 16, 33, 100]
+    k, v = (torch.randn(P, page, nkv, d, device=DEV, generator=g).to(BF) for _ in range(2))
+    table = torch.full((R, 12), -1, dtype=torch.int32, device=DEV)
+    ids = list(range(P))
+    for r, n in enumerate(start):
+        for j in range(-(-n // page)):
+            table[r, j] = ids.pop()
+    free = i32(*ids)
+    one, ctx, left = i32(*[1] * R), i32(*start), i32(len(ids), 0)
+    q, kn, vn = (torch.randn(R, h, d, device=DEV, generator=g).to(BF) for h in (nh, nkv, nkv))
+    logits, hist = torch.randn(R, V, device=DEV, generator=g), torch.randint(0, V, (R, 200), device=DEV, generator=g)
+    long = i32(20000)
+    kl, vl, tl = pool([20000], page, nkv, d, BF, g)
+
+    def step():
+        p = ops.paged_plan(one, ctx, table, free, left, page, R)
+        ops.paged_append(k, v, kn, vn, p.slots)
+        o = ops.paged_attention(q, k, v, table, p.cu_q, p.kv_lens, max_q=1)
+        o2 = ops.paged_attention(q[:1], kl, vl, tl, i32_zero_one, long, max_q=1)
+        y = ops.penalize_logits(logits, hist, None, p.kv_lens, repetition=1.3, frequency=0.1)
+        ctx.copy_(p.kv_lens)
+        left.copy_(p.free_left)
+        return o, o2, y
+
+    i32_zero_one = i32(0, 1)
+    keep = (ctx.clone(), left.clone(), table.clone(), k.clone(), v.clone())
+
+    def restore():
+        for a, b in zip((ctx, left, table, k, v), keep):
+            a.copy_(b)
+
+    want = []
+    for t in range(20):
+        q.fill_(0.1 * (t % 3 - 1)).add_(kn[:, :1])
+        kn.mul_(-1)
+        want.append([x.clone() for x in step()])
+    for t in range(20):
+        kn.mul_(-1)
+    restore()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    restore()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step()
+        graphs.append((graph, res))
+    restore()
+    for t in range(20):
+        q.fill_(0.1 * (t % 3 - 1)).add_(kn[:, :1])
+        kn.mul_(-1)
+        graph, res = graphs[t % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want[t])), t
+        (torch.randn(1000, device=DEV) @ torch.randn(1000, 50, device=DEV)).sum().item()
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams do not share scratch memory."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    k, v, table = pool([30000, 9000], 16, 2, 128, BF, g)
+    q = torch.randn(2, 8, 128, device=DEV, generator=g).to(BF)
+    q2 = torch.randn(2, 8, 128, device=DEV, generator=g).to(BF)
+    cu, kv = i32(0, 1, 2), i32(30000, 9000)
+    want, want2 = (ops.paged_attention(x, k, v, table, cu, kv, max_q=1) for x in (q, q2))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for s, (st, x) in enumerate(zip(streams, (q, q2))):
+            with torch.cuda.stream(st):
+                got[s].append(ops.paged_attention(x, k, v, table, cu, kv, max_q=1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got[0]) and all(torch.equal(o, want2) for o in got[1])
+
+
+def test_same_result_every_time():
+    g = torch.Generator(device=DEV).manual_seed(9)
+    qn, ctx = [1, 200, 1, 40], [9000, 800, 3, 4000]
+    kv = [a + b for a, b in zip(qn, ctx)]
+    k, v, table = pool(kv, 16, 2, 128, BF, g)
+    q = torch.randn(sum(qn), 8, 128, device=DEV, generator=g).to(BF)
+    cu = i32(0, 1, 201, 202, 242)
+    first = ops.paged_attention(q, k, v, table, cu, i32(*kv))
+    for _ in range(5):
+        assert torch.equal(ops.paged_attention(q, k, v, table, cu, i32(*kv)), first)
+
+
+def test_refusals_on_the_gpu():
+    t = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    one, cu = i32(1), i32(0, 1)
+    k, q = torch.zeros(2, 4, 1, 8, device=DEV), torch.zeros(1, 2, 8, device=DEV)
+    v = k.clone()
+    row = torch.zeros(1, 1, 8, device=DEV)
+    lg = torch.zeros(2, 40, device=DEV)
+    bad = [
+        lambda: ops.paged_plan(one.long(), one, t, one, one, 4, 1), lambda: ops.paged_plan(one, i32(1, 2), t, one, one, 4, 1),
+        lambda: ops.paged_plan(one, one, t, one, one, 0, 1), lambda: ops.paged_plan(one, one, t, one, one, 4, -1),
+        lambda: ops.paged_plan(one, one, t.view(-1), one, one, 4, 1), lambda: ops.paged_plan(one, one, t, one, i32(), 4, 1),
+        lambda: ops.paged_plan(one, one, t.cpu(), one, one, 4, 1), lambda: ops.paged_plan(one, one, t, one.cpu(), one, 4, 1),
+        lambda: ops.paged_append(k, v, row.expand(1, 2, 8), row, one), lambda: ops.paged_append(k, v, row.half(), row, one),
+        lambda: ops.paged_append(k, v, row, row, i32(1, 2)), lambda: ops.paged_append(k, k, row, row, one),
+        lambda: ops.paged_append(k, v, row, row, one.cpu()), lambda: ops.paged_append(k.double(), v.double(), row.double(), row.double(), one),
+        lambda: ops.paged_append(k[:, :1].expand(2, 4, 1, 8), v, row, row, one),
+        lambda: ops.paged_attention(q[..., :4], k, v, t, cu, one), lambda: ops.paged_attention(q, k, v, t, cu, i32(1, 1)),
+        lambda: ops.paged_attention(q, k, v, t.long(), cu, one), lambda: ops.paged_attention(q, k, v, t, cu, one, window=0),
+        lambda: ops.paged_attention(q, k, v, t, cu, one, out=q), lambda: ops.paged_attention(q.half(), k, v, t, cu, one),
+        lambda: ops.paged_attention(q, k, v, t, cu.cpu(), one), lambda: ops.paged_attention(q, k.cpu(), v, t, cu, one),
+        lambda: ops.paged_attention(q, k, v, t, cu, one, scale=math.inf),
+        lambda: ops.paged_attention(q, k, v, t, cu, one, out=torch.zeros(1, 1, 8, device=DEV).expand(1, 2, 8)),
+        lambda: ops.paged_attention(q.double(), k.double(), v.double(), t, cu, one),
+        lambda: ops.penalize_logits(lg[0]), lambda: ops.penalize_logits(lg, torch.zeros(1, 3, dtype=torch.int64, device=DEV)),
+        lambda: ops.penalize_logits(lg, torch.zeros(2, 3, device=DEV)), lambda: ops.penalize_logits(lg, bias=lg[:, :3]),
+        lambda: ops.penalize_logits(lg, bias=lg.half()), lambda: ops.penalize_logits(lg, allowed=i32(0)),
+        lambda: ops.penalize_logits(lg, out=lg[:, :39]), lambda: ops.penalize_logits(lg.double()),
+        lambda: ops.penalize_logits(lg, total_lens=i32(1, 2, 3)), lambda: ops.penalize_logits(lg, repetition=torch.ones(2)),
+    ]
+    for i, call in enumerate(bad):
+        try:
+            call()
+        except RuntimeError:
+            continue
+        pytest.fail(f"call {i} was not refused")
