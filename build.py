@@ -31,7 +31,7 @@ EXTRA_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "paged_plan.hip": _NO_PACKED_FP32,
     "paged_append.hip": _NO_PACKED_FP32,
-    "paged_attn.hip": _NO_PACKED_FP32,
+    "paged_attn.hip": [*_NO_PACKED_FP32, "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "penalties.hip": _NO_PACKED_FP32,
 }
 # Sources that textually include another source (rebuilt when that one changes).

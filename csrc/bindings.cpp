@@ -1468,7 +1468,10 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.max_q = (int)std::min<int64_t>(max_q > 0 ? max_q : N, N);
   a.type = type;
   a.zero_rest = !out.has_value();
-  dpa::paged_attn(a, cur_stream());
+  const size_t scratch = dpa::paged_attn_workspace(a, gemm_cus());
+  Tensor ws;
+  if (scratch > 0) ws = at::empty({(int64_t)scratch}, q.options().dtype(at::kByte));
+  dpa::paged_attn(a, gemm_cus(), scratch > 0 ? ws.data_ptr() : nullptr, cur_stream());
   return out.has_value() ? Tensor() : o;
 }
 

@@ -357,7 +357,9 @@ struct PagedAttnArgs {
   int type;          // kTypeBf16 / kTypeHalf / kTypeFloat
   bool zero_rest;    // rows outside every sequence: true = zeroed, false = left as they are
 };
-void paged_attn(const PagedAttnArgs& a, hipStream_t st);
+// scratch of one call: nothing in it outlives the call, and it need not be cleared
+size_t paged_attn_workspace(const PagedAttnArgs& a, int num_cus);
+void paged_attn(const PagedAttnArgs& a, int num_cus, void* workspace, hipStream_t st);
 
 // ---- Logit penalties (csrc/penalties.hip) -----------------------------------------------------
 struct PenaltyArgs {

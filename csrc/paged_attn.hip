@@ -7,6 +7,10 @@
 //
 // Any type, width (<= 256) and stride: one wave per (row, head). Lane = key for the scores of 64 keys at a time, then
 // lane = feature for the values, probabilities by broadcast; running maximum, sum and output in fp32.
+#include <algorithm>
+#include <cmath>
+
+#include "mfma_tiles.h"
 #include "paged.h"
 
 namespace dpa {
@@ -97,10 +101,832 @@ __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAt
     if (j < nd && lane + 64 * j < a.width) Cvt<T>::st(o + lane + 64 * j, l == 0.f ? 0.f : acc[j] * inv);
 }
 
+
+// ---------------------------------------------------------------------------------------------------------
+// bf16 / fp16, widths up to 128 in whole 16-byte pieces: matrix instructions.
+//
+// The G = nh / nkv query heads of a KV head share its keys, so a request's rows are (token, head of the group) pairs
+// packed per KV head; K and V are read once per tile of rows, not once per head. An item is (request, row tile, KV
+// head, piece of the keys):
+//   few rows (at most 32 packed, a decode step): the four waves of a workgroup take 32-key subtiles in turn, each
+//     through its own part of LDS without any workgroup barrier, and are merged at the end. Bound by K / V bytes.
+//   chunks: 128 packed rows, 32 per wave, over 64-key tiles that the waves share (two stages). Bound by products.
+// Both use the same step: S^T = K Q^T (v_mfma 32x32x16, lane = row, keys along the accumulator), running maximum and
+// sum per lane, O^T += V^T P^T with V read transposed from LDS.
+//
+// Lengths live on the device, so every workgroup derives the list of items from them (one pass over the requests:
+// R <= 256 is one load per thread) and takes the one of its number. The keys of a request are cut into pieces when
+// there are fewer items than `target`; the pieces leave (O, reference, sum) in the workspace and a second kernel joins
+// them, in the order of the keys, so a result does not depend on which workgroup ran when.
+//
+// The score's reference point mb (log2 units) moves only when a subtile's maximum passes it by 2^8: p <= 2^(kBias + 8).
+// kBias = 6 for fp16 keeps small probabilities out of its subnormal range (one of 2^-20 still has all its bits).
+// Scores are scaled in fp32 after the product: q keeps its bits. A negative scale negates q, which is exact.
+// ---------------------------------------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFewRows = 32, kChunkRows = 128, kThreads = 256;
+constexpr int kFewStep = 128, kChunkStep = 64;      // keys a workgroup advances by: pieces are multiples of it
+
+template <typename T> struct Frag;
+template <> struct Frag<bf16_t> {
+  static constexpr int kBias = 0;
+  static constexpr unsigned kExp = 0x7f807f80u, kExpOne = 0x00800080u, kInf = 0x7f80u, kSign = 0x8000u;
+  static constexpr unsigned kOne = 0x3f80u, k64 = 0x4280u, k4096 = 0x4580u;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfrag, a), __builtin_bit_cast(bfrag, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+template <> struct Frag<half_t> {
+  static constexpr int kBias = 6;
+  static constexpr unsigned kExp = 0x7c007c00u, kExpOne = 0x04000400u, kInf = 0x7c00u, kSign = 0x8000u;
+  static constexpr unsigned kOne = 0x3c00u, k64 = 0x5400u, k4096 = 0x6c00u;
+  typedef __attribute__((ext_vector_type(8))) _Float16 half8;
+  typedef __attribute__((ext_vector_type(2))) _Float16 half2_t;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack(float lo, float hi) {
+    half2_t v;
+    v[0] = (half_t)lo;     // round to nearest even
+    v[1] = (half_t)hi;
+    return __builtin_bit_cast(unsigned, v);
+  }
+};
+
+struct FastArgs {
+  float c;             // |scale| log2 e
+  bool negate;         // scale < 0
+  int G;               // query heads per KV head
+  FastDiv by_group;
+  int target;          // items wanted on the card
+  int max_items, max_slots, slot_rows;
+  float* part;         // [max_slots][slot_rows][W] unnormalised outputs of pieces
+  float* ml;           // [max_slots][slot_rows][2] reference, sum
+  int* meta;           // [max_slots][8]
+  int* header;         // [0] = slots in use
+};
+
+// 256 zero bytes: what rows that no query may see, and pages that do not exist, read as
+__device__ __attribute__((aligned(256))) const unsigned zero_row[64] = {};
+
+struct Request {
+  int start, n;        // its rows of the batch
+  int shift;           // position of batch row i: i + shift
+  int rows, tiles;     // packed rows per KV head and tiles of them
+  int klo, khi;        // keys that any of its rows sees
+  bool chunk;
+};
+__device__ __forceinline__ Request request(const PagedAttnArgs& a, const FastArgs& f, int r) {
+  Request q;
+  const int c0 = a.cu_q[r], c1 = a.cu_q[r + 1];
+  q.start = min(max(c0, 0), a.N);
+  q.n = min(max(c1, q.start), a.N) - q.start;
+  const long long sh = (long long)a.kv_lens[r] - c1;
+  q.shift = (int)min(max(sh, -(1ll << 30)), 1ll << 30);
+  q.rows = q.n * f.G;
+  q.chunk = q.rows > kFewRows;
+  q.tiles = q.chunk ? (q.rows + kChunkRows - 1) / kChunkRows : (q.rows > 0 ? 1 : 0);
+  const int cap = a.M * a.page;
+  q.khi = min(q.start + q.n + q.shift, cap);
+  q.klo = a.window > 0 ? max(q.start + q.shift - a.window + 1, 0) : 0;
+  if (q.khi < q.klo) q.khi = q.klo;
+  return q;
+}
+
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_dma_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// 1 KiB global -> LDS, one 16-byte piece per lane: from a scalar base plus the lane's offset, or from the lane's address.
+__device__ __forceinline__ void dma_uniform(unsigned long long base, unsigned voff, unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %2"
+      :
+      : "v"(voff), "s"(dst), "s"(base)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void dma_lane(unsigned long long addr, unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, off"
+      :
+      : "v"(addr), "s"(dst)
+      : "memory", "m0");
+}
+
+// Rows of pages -> LDS. A piece is RPP rows of W columns. When the page size is a multiple of RPP and the row fills the
+// tile (UNI), a piece lies in one page: the page number and the address come from scalar registers.
+template <int W, int NP, bool UNI>
+struct PageRows {
+  static constexpr int CPR = W / 8, RPP = 64 / CPR;
+  static constexpr int VAR = W == 128 ? 4 : 2;      // the swizzle of a piece repeats after VAR pieces
+  const PagedAttnArgs* a;
+  const int* table;       // the request's row
+  unsigned long long kb, vb;
+  int klo, khi, lane;
+  bool checked;           // every page of the range exists
+  unsigned kv_off[2][VAR];
+  int pg[NP];
+
+  __device__ __forceinline__ void init(const PagedAttnArgs& args, const int* t, int g, int lo, int hi, bool ok, int lane_) {
+    a = &args;
+    table = t;
+    klo = lo;
+    khi = hi;
+    checked = ok;
+    lane = lane_;
+    kb = (unsigned long long)args.k + 2ull * (unsigned long long)(g * args.k_hs);
+    vb = (unsigned long long)args.v + 2ull * (unsigned long long)(g * args.v_hs);
+#pragma unroll
+    for (int v = 0; v < VAR; ++v) {
+      const int row = v * RPP + lane / CPR;
+      const unsigned col = 16u * swz<W>(row, lane % CPR);
+      kv_off[0][v] = (unsigned)(lane / CPR) * (unsigned)(2 * args.k_rs) + col;
+      kv_off[1][v] = (unsigned)(lane / CPR) * (unsigned)(2 * args.v_rs) + col;
+    }
+  }
+  __device__ __forceinline__ bool whole(int ks0) const { return UNI && checked && ks0 >= klo && ks0 + NP * RPP <= khi; }
+  // page numbers of the rows [ks0, ks0 + NP * RPP), for the issue() of those rows
+  __device__ __forceinline__ void fetch(int ks0) {
+    if (!whole(ks0)) return;
+#pragma unroll
+    for (int pc = 0; pc < NP; ++pc) {
+      const int col = fast_div(ks0 + pc * RPP, a->by_page);
+      typedef const __attribute__((address_space(4))) int* scalar_ptr;
+      pg[pc] = *(scalar_ptr)(unsigned long long)(table + __builtin_amdgcn_readfirstlane(col));
+    }
+  }
+  template <bool V>
+  __device__ __forceinline__ void issue(int ks0, unsigned lds) const {
+    const unsigned long long base = V ? vb : kb;
+    const unsigned long long ps = 2ull * (unsigned long long)(V ? a->v_ps : a->k_ps);
+    const unsigned rs = 2u * (unsigned)(V ? a->v_rs : a->k_rs);
+    if (whole(ks0)) {
+#pragma unroll
+      for (int pc = 0; pc < NP; ++pc) {
+        const int key = ks0 + pc * RPP;
+        const int row = __builtin_amdgcn_readfirstlane(key - fast_div(key, a->by_page) * a->page);
+        dma_uniform(base + (unsigned)pg[pc] * ps + (unsigned)row * rs, kv_off[V][pc % VAR], lds + pc * 1024);
+      }
+      return;
+    }
+#pragma unroll
+    for (int pc = 0; pc < NP; ++pc) {
+      const int row = pc * RPP + lane / CPR, key = ks0 + row;
+      const int ch = swz<W>(row, lane % CPR);
+      unsigned long long addr = (unsigned long long)zero_row + 16u * ch;
+      if (key >= klo && key < khi) {
+        const int col = fast_div(key, a->by_page);
+        const int p = table[col];
+        if (p >= 0 && p < a->pages && ch * 8 < a->width)
+          addr = base + (unsigned)p * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
+      }
+      dma_lane(addr, lds + pc * 1024);
+    }
+  }
+};
+
+// One lane's row: bounds of the keys it sees, reference, sum (of its half of the keys) and the output tile.
+template <int W>
+struct RowState {
+  int lo, hi;
+  float mb, l;
+  f32x16 o[W / 32];
+  __device__ __forceinline__ void clear() {
+    mb = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < W / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+  }
+};
+
+__device__ __forceinline__ void swap_halves(float& x, float& y) {
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 0" : "+v"(x), "+v"(y));
+}
+__device__ __forceinline__ float max_halves(float x) {
+  float u = x, v = x;
+  swap_halves(u, v);
+  return fmaxf(u, v);
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  float u = x, v = x;
+  swap_halves(u, v);
+  return u + v;
+}
+
+// Values that are not finite, in a subtile some of whose keys are hidden from some rows: 0 * inf would reach those rows.
+// They leave the fragments, and a product of the visibility (0 / 1) with codes (1: +inf, 64: -inf, 4096: NaN; at most 32
+// keys, so the counts do not run into each other) says which outputs they belong in.
+template <typename T, int W>
+__device__ __forceinline__ void place_non_finite(u32x4 (&vf)[2][W / 32], f32x16 (&o)[W / 32], int lo_rel, int hi_rel, int hh) {
+  typedef Frag<T> F;
+  u32x4 seen[2];
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unsigned w = 0u;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int key = acc_row(8 * s2 + 2 * j + e, hh);
+        if (key >= lo_rel && key <= hi_rel) w |= F::kOne << (16 * e);
+      }
+      seen[s2][j] = w;
+    }
+#pragma unroll
+  for (int dt = 0; dt < W / 32; ++dt) {
+    f32x16 code;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) code[i] = 0.f;
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      u32x4 cw;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unsigned w = vf[s2][dt][j], keep = w, c = 0u;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned x = (w >> (16 * e)) & 0xffffu;
+          if ((x & F::kInf) == F::kInf) {
+            keep &= ~(0xffffu << (16 * e));
+            c |= ((x & 0x7fffu) != F::kInf ? F::k4096 : (x & F::kSign) ? F::k64 : F::kOne) << (16 * e);
+          }
+        }
+        vf[s2][dt][j] = keep;
+        cw[j] = c;
+      }
+      code = F::mfma(cw, seen[s2], code);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int n = (int)code[i];
+      if (n != 0) {
+        const bool pos = (n & 63) != 0, neg = (n & 4032) != 0;
+        o[dt][i] += n >= 4096 || (pos && neg) ? __builtin_nanf("") : (pos ? INFINITY : -INFINITY);
+      }
+    }
+  }
+}
+
+// A 32-key subtile: keys [ks0, ks0 + 32) in the LDS tiles kt, vt. mask: some of them are hidden from some row of the wave.
+template <typename T, int W, class AfterK, class BeforeV, class AfterV, class Hidden>
+__device__ __forceinline__ void subtile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
+                                        RowState<W>& st, int lane, AfterK after_k, BeforeV before_v, AfterV after_v,
+                                        Hidden hidden) {
+  typedef Frag<T> F;
+  constexpr int NK = W / 16, ND = W / 32;
+  const int r = lane & 31, hh = lane >> 5;
+  u32x4 kf[NK];
+#pragma unroll
+  for (int ks = 0; ks < NK; ++ks) kf[ks] = __builtin_bit_cast(u32x4, row_frag<W>(kt, r, ks, hh));
+  after_k();
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < NK; ++ks) s = F::mfma(kf[ks], qf[ks], s);
+  const int lo_rel = st.lo - ks0, hi_rel = st.hi - ks0;
+  if (mask) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = acc_row(i, hh);
+      if (key < lo_rel || key > hi_rel) s[i] = -INFINITY;
+    }
+    hidden(s);
+  }
+  float mx = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+  mx = max_halves(mx) * c;
+  const bool move = mx > st.mb + (float)(F::kBias + 8);      // the first key a row sees moves it from -inf
+  if (__any(move)) {
+    const float to = mx - (float)F::kBias;
+    const float alpha = move ? __builtin_amdgcn_exp2f(st.mb - to) : 1.f;
+    st.mb = move ? to : st.mb;
+    st.l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[dt][i] *= alpha;
+  }
+  before_v();
+  u32x4 vf[2][ND];
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) vf[s2][dt] = __builtin_bit_cast(u32x4, tr_frag<W>(vt, 0, s2, dt, lane));
+  const float base = st.mb == -INFINITY ? 0.f : st.mb;       // no key seen yet: every s is -inf
+  float rs = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));
+    rs += s[i];
+  }
+  st.l += rs;
+  after_v();
+  if (mask) {
+    unsigned bad = 0u;
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (vf[s2][dt][j] & F::kExp) + F::kExpOne;
+    if (__any((bad & 0x80008000u) != 0u)) place_non_finite<T, W>(vf, st.o, lo_rel, hi_rel, hh);
+  }
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2) {
+    u32x4 pb;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pb[j] = F::pack(s[8 * s2 + 2 * j], s[8 * s2 + 2 * j + 1]);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) st.o[dt] = F::mfma(vf[s2][dt], pb, st.o[dt]);
+  }
+}
+
+// fp32 output tile [32 rows][W] of a wave in LDS; 16-byte pieces XORed with the row against bank conflicts.
+template <int W>
+__device__ __forceinline__ float* o_piece(char* tile, int row, int piece) {
+  return reinterpret_cast<float*>(tile + row * (W * 4) + 16 * (piece ^ (row & (W / 4 - 1))));
+}
+
+template <typename T, int W, bool UNI>
+__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
+  constexpr int NK = W / 16, ND = W / 32, SUB = 32 * W * 2, REGION = 4 * SUB / 2;   // REGION: a wave's 32 x W fp32 = 2 SUB
+  static_assert(REGION == 2 * SUB, "one K and one V subtile per wave");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red_f[4];
+  __shared__ int red_i[4], red_s[4], found[8];
+  __shared__ float ml_s[4][32][2];
+  const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
+
+  // ---- rows outside every sequence ----
+  if (a.zero_rest) {
+    const int lo = a.R > 0 ? min(max(a.cu_q[0], 0), a.N) : a.N, hi = a.R > 0 ? min(max(a.cu_q[a.R], 0), a.N) : a.N;
+    const int rest = lo + a.N - max(hi, lo);
+    const long long total = (long long)rest * a.nh * a.width;
+    for (long long i = (long long)blockIdx.x * kThreads + tid; i < total; i += (long long)gridDim.x * kThreads) {
+      const int d = (int)(i % a.width), h = (int)((i / a.width) % a.nh);
+      int row = (int)(i / a.width / a.nh);
+      if (row >= lo) row += max(hi, lo) - lo;
+      ((uint16_t*)a.o)[(long long)row * a.o_ts + (long long)h * a.o_hs + d] = 0;
+    }
+  }
+
+  // ---- this workgroup's item ----
+  const int per = (a.R + kThreads - 1) / kThreads;      // consecutive requests per thread
+  const int ra = min(tid * per, a.R), rb = min(ra + per, a.R);
+  float cost = 0.f;
+  for (int r = ra; r < rb; ++r) {
+    const Request q = request(a, f, r);
+    cost += (float)q.tiles * (float)(q.khi - q.klo) * (q.chunk ? 2.f : 1.f);
+  }
+  cost = wave_sum(cost);
+  if (lane == 0) red_f[wave] = cost;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  const float budget = (red_f[0] + red_f[1] + red_f[2] + red_f[3]) * (float)a.nkv / (float)f.target;
+  const int few_keys = max((int)fminf(budget / (float)kFewStep, 8e6f) + 1, 2) * kFewStep;
+  const int chunk_keys = max((int)fminf(budget * 0.5f / (float)kChunkStep, 8e6f) + 1, 8) * kChunkStep;
+  auto pieces = [&](const Request& q) {
+    const int len = q.khi - q.klo, step = q.chunk ? chunk_keys : few_keys;
+    return len <= step ? 1 : (len + step - 1) / step;
+  };
+  int items = 0, slots = 0;
+  for (int r = ra; r < rb; ++r) {
+    const Request q = request(a, f, r);
+    const int np = pieces(q), k = q.tiles * np * a.nkv;
+    items += k;
+    if (np > 1) slots += k;
+  }
+  int pi = items, ps = slots;     // inclusive prefixes over the threads
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int x = __shfl_up(pi, off, 64), y = __shfl_up(ps, off, 64);
+    if (lane >= off) {
+      pi += x;
+      ps += y;
+    }
+  }
+  if (lane == 63) {
+    red_i[wave] = pi;
+    red_s[wave] = ps;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    if (w < wave) {
+      pi += red_i[w];
+      ps += red_s[w];
+    }
+  pi -= items;
+  ps -= slots;
+  const int id = blockIdx.x;
+  if (id == 0 && tid == kThreads - 1 && f.header != nullptr) f.header[0] = min(ps + slots, f.max_slots);
+  if (id >= pi && id < pi + items) {
+    for (int r = ra; r < rb; ++r) {
+      const Request q = request(a, f, r);
+      const int np = pieces(q), k = q.tiles * np * a.nkv;
+      if (id < pi + k) {
+        found[0] = r;
+        found[1] = id - pi;
+        found[2] = ps + id - pi;
+        found[3] = np;
+        break;
+      }
+      pi += k;
+      if (np > 1) ps += k;
+    }
+  }
+  __syncthreads();
+  const int r = __builtin_amdgcn_readfirstlane(found[0]);
+  if (r < 0) return;
+  const Request q = request(a, f, r);
+  const int np = __builtin_amdgcn_readfirstlane(found[3]), slot = __builtin_amdgcn_readfirstlane(found[2]);
+  int j = __builtin_amdgcn_readfirstlane(found[1]);
+  const int g = j % a.nkv;
+  j /= a.nkv;
+  const int piece = j % np;
+  const int tile = q.tiles - 1 - j / np;                 // the rows that see most come first
+  if (tile < 0 || j < 0 || (np > 1 && (unsigned)slot >= (unsigned)f.max_slots)) return;   // lengths that contradict each other
+  const int rows0 = tile * kChunkRows, nrows = min(q.chunk ? kChunkRows : kFewRows, q.rows - rows0);
+  const int t_first = fast_div(rows0, f.by_group), t_last = fast_div(rows0 + nrows - 1, f.by_group);
+  const int p_first = q.start + t_first + q.shift, p_last = q.start + t_last + q.shift, cap = a.M * a.page;
+  const int khi = max(min(p_last + 1, cap), 0), klo = min(a.window > 0 ? max(p_first - a.window + 1, 0) : 0, khi);
+  const int step = q.chunk ? kChunkStep : kFewStep;
+  const int k_base = klo & ~63;
+  const int span = ((khi - k_base + np - 1) / np + step - 1) / step * step;
+  const int k0 = k_base + piece * span, k1 = min(khi, k0 + span);
+
+  // ---- do all pages of the piece exist? ----
+  const int* table = a.table + (long long)r * a.table_ld;
+  bool missing = false;
+  if (k1 > k0) {
+    const int c_lo = fast_div(max(k0, klo), a.by_page), c_hi = fast_div(k1 - 1, a.by_page);
+    for (int col = c_lo + tid; col <= c_hi; col += kThreads) missing |= (unsigned)table[col] >= (unsigned)a.pages;
+  }
+  missing = __syncthreads_or(missing);
+
+  // ---- queries of this lane's row ----
+  const int row = rows0 + (q.chunk ? wave * 32 : 0) + r32;
+  const bool valid = row < q.rows && (q.chunk || r32 < nrows);
+  const int tok = fast_div(valid ? row : 0, f.by_group), head = g * f.G + (valid ? row - tok * f.G : 0);
+  u32x4 qf[NK];
+  {
+    const uint16_t* qp = (const uint16_t*)a.q + (long long)(q.start + tok) * a.q_ts + (long long)head * a.q_hs;
+    const unsigned flip = f.negate ? 0x80008000u : 0u;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+      const int d = ks * 16 + hh * 8;
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (valid && d < a.width) {
+        v = *reinterpret_cast<const u32x4*>(qp + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] ^= flip;
+      }
+      qf[ks] = v;
+    }
+  }
+  RowState<W> st;
+  st.clear();
+  {
+    const int pos = q.start + tok + q.shift;
+    st.hi = valid ? min(pos, cap - 1) : -1;
+    st.lo = a.window > 0 ? pos - a.window + 1 : 0;
+  }
+  auto hide_missing = [&](int ks0) {
+    return [=](f32x16& s) {
+      if (!missing) return;
+#pragma unroll 1
+      for (int i = 0; i < 32; ++i) {     // one page number at a time, the same for all lanes
+        const int key = ks0 + i;
+        bool gone = true;
+        if (key < khi) gone = (unsigned)table[fast_div(key, a.by_page)] >= (unsigned)a.pages;
+        if (gone) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (acc_row(e, hh) == i) s[e] = -INFINITY;
+        }
+      }
+    };
+  };
+
+  if (!q.chunk) {
+    // ---- few rows: subtile t of the piece belongs to wave t % 4 ----
+    constexpr int NP = SUB / 1024;
+    char* const kt = smem + wave * REGION;
+    char* const vt = kt + SUB;
+    const unsigned k_lds = lds0 + wave * REGION, v_lds = k_lds + SUB;
+    PageRows<W, NP, UNI> pr;
+    pr.init(a, table, g, klo, khi, !missing, lane);
+    int ks0 = k0 + wave * 32;
+    if (ks0 < k1) {
+      pr.fetch(ks0);
+      pr.template issue<false>(ks0, k_lds);
+      pr.template issue<true>(ks0, v_lds);
+    }
+    for (; ks0 < k1; ks0 += 128) {
+      const int next = ks0 + 128;
+      const bool more = next < k1;
+      const bool mask = missing || ks0 + 31 > p_first || ks0 + 32 > cap || (a.window > 0 && ks0 < p_last - a.window + 1);
+      if (more) pr.fetch(next);
+      wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
+      subtile<T, W>(
+          kt, vt, ks0, mask, f.c, qf, st, lane,
+          [&]() {
+            wait_lds();         // the key fragments are in registers: their place takes the next subtile's
+            if (more) pr.template issue<false>(next, k_lds);
+          },
+          [&]() {
+            if (more) wait_dma_but<NP>();
+            else wait_dma_but<0>();
+          },
+          [&]() {
+            wait_lds();
+            if (more) pr.template issue<true>(next, v_lds);
+          },
+          hide_missing(ks0));
+    }
+    // ---- merge the waves ----
+    const float l = sum_halves(st.l);
+    if (hh == 0) {
+      ml_s[wave][r32][0] = st.mb;
+      ml_s[wave][r32][1] = l;
+    }
+    __syncthreads();
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (ml_s[w][r32][1] != 0.f) M = fmaxf(M, ml_s[w][r32][0]);
+    const float scale = l != 0.f ? __builtin_amdgcn_exp2f(st.mb - M) : 0.f;
+    char* const tile_o = smem + wave * REGION;
+    if (valid) {
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = l != 0.f ? st.o[dt][4 * g4 + e] * scale : 0.f;
+          *reinterpret_cast<f32x4*>(o_piece<W>(tile_o, r32, 8 * dt + 2 * g4 + hh)) = v;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < nrows * (W / 8); i += kThreads) {
+      const int rr = i / (W / 8), d8 = i % (W / 8);
+      float M2 = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (ml_s[w][rr][1] != 0.f) M2 = fmaxf(M2, ml_s[w][rr][0]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (ml_s[w][rr][1] != 0.f) L += ml_s[w][rr][1] * __builtin_amdgcn_exp2f(ml_s[w][rr][0] - M2);
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(o_piece<W>(smem + w * REGION, rr, 2 * d8));
+        const f32x4 y = *reinterpret_cast<const f32x4*>(o_piece<W>(smem + w * REGION, rr, 2 * d8 + 1));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[e] += x[e];
+          o[4 + e] += y[e];
+        }
+      }
+      if (np > 1) {
+        float* dst = f.part + ((long long)slot * f.slot_rows + rr) * W + 8 * d8;
+        store8(dst, o);
+        if (d8 == 0) {
+          f.ml[((long long)slot * f.slot_rows + rr) * 2] = M2;
+          f.ml[((long long)slot * f.slot_rows + rr) * 2 + 1] = L;
+        }
+      } else if (8 * d8 < a.width) {
+        const float inv = L != 0.f ? 1.f / L : 0.f;
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = L != 0.f ? Frag<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
+        const int tk = fast_div(rows0 + rr, f.by_group), hd = g * f.G + rows0 + rr - tk * f.G;
+        *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(q.start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
+      }
+    }
+  } else {
+    // ---- chunks: the waves share 64-key tiles ----
+    constexpr int NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;    // pieces per wave; K and V tile
+    PageRows<W, NP, UNI> pr;
+    pr.init(a, table, g, klo, khi, !missing, lane);
+    constexpr int WROWS = 16;       // rows of a tile that a wave transfers
+    const int w_off = wave * WROWS;
+    const unsigned w_lds = lds0 + wave * NP * 1024;
+    const int wt_first = fast_div(min(rows0 + wave * 32, q.rows - 1), f.by_group);
+    const int wt_last = fast_div(min(rows0 + wave * 32 + 31, q.rows - 1), f.by_group);
+    const int wp_first = q.start + wt_first + q.shift, wp_last = q.start + wt_last + q.shift;
+    const bool wave_live = rows0 + wave * 32 < q.rows;
+    if (k0 < k1) {
+      pr.fetch(k0 + w_off);
+      pr.template issue<false>(k0 + w_off, w_lds);
+      pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
+    }
+    int stage = 0;
+    if (k0 + 64 < k1) pr.fetch(k0 + 64 + w_off);
+    for (int kt0 = k0; kt0 < k1; kt0 += 64) {
+      wait_dma_but<0>();
+      __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
+      const int next = kt0 + 64;
+      if (next < k1) {
+        const unsigned nb = w_lds + (stage ^ 1) * STAGE;
+        pr.template issue<false>(next + w_off, nb);
+        pr.template issue<true>(next + w_off, nb + 2 * SUB);
+        if (next + 64 < k1) pr.fetch(next + 64 + w_off);
+      }
+      const char* const kt = smem + stage * STAGE;
+      const char* const vt = kt + 2 * SUB;
+      stage ^= 1;
+      if (!wave_live) continue;
+#pragma unroll 1
+      for (int sub = 0; sub < 2; ++sub) {
+        const int ks0 = kt0 + 32 * sub;
+        if (ks0 > wp_last || ks0 >= khi) break;
+        if (a.window > 0 && ks0 + 31 < wp_first - a.window + 1) continue;
+        const bool mask = missing || ks0 + 31 > wp_first || ks0 + 32 > cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
+        subtile<T, W>(kt + sub * SUB, vt + sub * SUB, ks0, mask, f.c, qf, st, lane, [] {}, [] {}, [] {}, hide_missing(ks0));
+      }
+    }
+    const float l = sum_halves(st.l);
+    __syncthreads();          // every wave is done with the tiles
+    char* const tile_o = smem + wave * REGION;
+    const float inv = np > 1 ? 1.f : (l != 0.f ? 1.f / l : 0.f);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = l != 0.f ? st.o[dt][4 * g4 + e] * inv : 0.f;
+        *reinterpret_cast<f32x4*>(o_piece<W>(tile_o, r32, 8 * dt + 2 * g4 + hh)) = v;
+      }
+    wait_lds();
+    const int mine = min(32, nrows - wave * 32);
+    for (int i = lane; i < mine * (W / 8); i += 64) {
+      const int rr = i / (W / 8), d8 = i % (W / 8);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(o_piece<W>(tile_o, rr, 2 * d8));
+      const f32x4 y = *reinterpret_cast<const f32x4*>(o_piece<W>(tile_o, rr, 2 * d8 + 1));
+      const int rw = wave * 32 + rr;
+      if (np > 1) {
+        float* dst = f.part + ((long long)slot * f.slot_rows + rw) * W + 8 * d8;
+        *reinterpret_cast<f32x4*>(dst) = x;
+        *reinterpret_cast<f32x4*>(dst + 4) = y;
+      } else if (8 * d8 < a.width) {
+        u32x4 w = {Frag<T>::pack(x[0], x[1]), Frag<T>::pack(x[2], x[3]), Frag<T>::pack(y[0], y[1]), Frag<T>::pack(y[2], y[3])};
+        const int tk = fast_div(rows0 + rw, f.by_group), hd = g * f.G + rows0 + rw - tk * f.G;
+        *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(q.start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
+      }
+    }
+    if (np > 1 && hh == 0 && r32 < mine) {
+      f.ml[((long long)slot * f.slot_rows + wave * 32 + r32) * 2] = st.mb;
+      f.ml[((long long)slot * f.slot_rows + wave * 32 + r32) * 2 + 1] = l;
+    }
+  }
+  if (np > 1 && tid == 0) {
+    int* m = f.meta + (long long)slot * 8;
+    m[0] = piece == 0 ? np : 0;      // the first piece of a tile leads the others, nkv slots apart
+    m[1] = q.start;
+    m[2] = rows0;
+    m[3] = nrows;
+    m[4] = g;
+  }
+}
+
+// The pieces of one row tile and KV head: o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, in the order of the keys.
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs a, FastArgs f) {
+  const int slot = blockIdx.x;
+  if (slot >= f.header[0]) return;
+  const int* m = f.meta + (long long)slot * 8;
+  const int np = m[0], start = m[1], rows0 = m[2], nrows = m[3], g = m[4];
+  if (np < 2) return;
+  for (int i = threadIdx.x; i < nrows * (W / 8); i += kThreads) {
+    const int rr = i / (W / 8), d8 = i % (W / 8);
+    if (8 * d8 >= a.width) continue;
+    float M = -INFINITY, L = 0.f, o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    for (int p = 0; p < np; ++p) {
+      const float* ml = f.ml + ((long long)(slot + p * a.nkv) * f.slot_rows + rr) * 2;
+      if (ml[1] != 0.f) M = fmaxf(M, ml[0]);
+    }
+    for (int p = 0; p < np; ++p) {
+      const long long at = (long long)(slot + p * a.nkv) * f.slot_rows + rr;
+      const float l = f.ml[at * 2 + 1];
+      if (l == 0.f) continue;
+      const float w = __builtin_amdgcn_exp2f(f.ml[at * 2] - M);
+      float x[8];
+      load8(f.part + at * W + 8 * d8, x);
+      L += l * w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += x[e] * w;
+    }
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = L != 0.f ? Frag<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
+    const int tk = fast_div(rows0 + rr, f.by_group), hd = g * f.G + rows0 + rr - tk * f.G;
+    *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
+  }
+}
+
+// Whether the matrix kernels take the call: 16-bit types, whole aligned 16-byte pieces, offsets inside a page below 2^32.
+bool fast_ok(const PagedAttnArgs& a) {
+  if (a.type == kTypeFloat || a.width % 8 != 0 || a.width > 128) return false;
+  const long long strides[] = {a.q_ts, a.q_hs, a.o_ts, a.o_hs, a.k_ps, a.k_rs, a.k_hs, a.v_ps, a.v_rs, a.v_hs};
+  for (long long s : strides)
+    if (s % 8 != 0 || s < 0) return false;
+  for (const void* p : {a.q, a.k, a.v, (const void*)a.o})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+  const long long lim = 1ll << 31;
+  return a.k_rs * 2 * std::max(a.page, 8) < lim && a.v_rs * 2 * std::max(a.page, 8) < lim;
+}
+
+struct Plan {
+  int target, grid, slots, slot_rows;
+  size_t part, ml, meta, total;
+};
+Plan plan_items(const PagedAttnArgs& a, int num_cus) {
+  Plan p;
+  const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
+  p.target = num_cus * 4;
+  // tiles: one per request with rows, and one more for every 128 rows of a chunk
+  const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
+  p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
+  p.slots = (int)std::min<long long>(2ll * p.target, p.grid);
+  p.slot_rows = (long long)a.N * G > kFewRows ? kChunkRows : kFewRows;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  p.part = up((size_t)p.slots * p.slot_rows * W * 4);
+  p.ml = up((size_t)p.slots * p.slot_rows * 8);
+  p.meta = up((size_t)p.slots * 32);
+  p.total = p.part + p.ml + p.meta + 256;
+  return p;
+}
+
+template <typename T, int W, bool UNI>
+void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
+  constexpr int lds = 4 * 2 * 32 * W * 2;
+  static bool set = false;       // above the default limit of dynamic LDS; the same value every time
+  if (!set) {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, W, UNI>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    set = true;
+  }
+  hipLaunchKernelGGL((paged_attn_kernel<T, W, UNI>), dim3(grid), dim3(kThreads), lds, st, a, f);
+  if (f.max_slots > 0) hipLaunchKernelGGL((paged_attn_join_kernel<T, W>), dim3(f.max_slots), dim3(kThreads), 0, st, a, f);
+}
+template <typename T>
+void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
+  if (a.width <= 64) {
+    if (a.width == 64 && a.page % 8 == 0) launch_fast<T, 64, true>(a, f, grid, st);
+    else launch_fast<T, 64, false>(a, f, grid, st);
+  } else {
+    if (a.width == 128 && a.page % 4 == 0) launch_fast<T, 128, true>(a, f, grid, st);
+    else launch_fast<T, 128, false>(a, f, grid, st);
+  }
+}
+
 }  // namespace
 
-void paged_attn(const PagedAttnArgs& a, hipStream_t st) {
+size_t paged_attn_workspace(const PagedAttnArgs& a, int num_cus) {
+  return a.N > 0 && a.R > 0 && fast_ok(a) ? plan_items(a, num_cus).total : 0;
+}
+
+void paged_attn(const PagedAttnArgs& a, int num_cus, void* workspace, hipStream_t st) {
   if (a.N == 0 || a.nh == 0) return;
+  if (workspace != nullptr) {
+    const Plan p = plan_items(a, num_cus);
+    FastArgs f{};
+    f.negate = a.scale < 0.f;
+    f.c = std::max(std::fabs(a.scale) * kLog2e, 1e-30f);      // a scale of 0: equal weights, and no 0 * inf at masked keys
+    f.G = a.nh / a.nkv;
+    f.by_group = make_fast_div(f.G);
+    f.target = p.target;
+    f.max_items = p.grid;
+    f.max_slots = p.slots;
+    f.slot_rows = p.slot_rows;
+    char* w = (char*)workspace;
+    f.part = (float*)w;
+    f.ml = (float*)(w + p.part);
+    f.meta = (int*)(w + p.part + p.ml);
+    f.header = (int*)(w + p.part + p.ml + p.meta);
+    if (a.type == kTypeBf16) launch_fast<bf16_t>(a, f, p.grid, st);
+    else launch_fast<half_t>(a, f, p.grid, st);
+    return;
+  }
   const long long waves = (long long)a.N * a.nh;
   const dim3 grid((unsigned)((waves + kGenWaves - 1) / kGenWaves)), block(kGenWaves * 64);
   if (a.type == kTypeBf16) hipLaunchKernelGGL((paged_attn_rows_kernel<bf16_t>), grid, block, 0, st, a);
