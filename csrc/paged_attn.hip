@@ -9,6 +9,7 @@
 // lane = feature for the values, probabilities by broadcast; running maximum, sum and output in fp32.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "mfma_tiles.h"
 #include "paged.h"
@@ -154,17 +155,20 @@ template <> struct Frag<half_t> {
   }
 };
 
+constexpr int kWaveRequests = 256;    // up to here every wave derives the items by itself
+
 struct FastArgs {
   float c;             // |scale| log2 e
   bool negate;         // scale < 0
   int G;               // query heads per KV head
   FastDiv by_group;
   int target;          // items wanted on the card
-  int max_items, max_slots, slot_rows;
+  int max_slots, slot_rows;
   float* part;         // [max_slots][slot_rows][W] unnormalised outputs of pieces
   float* ml;           // [max_slots][slot_rows][2] reference, sum
   int* meta;           // [max_slots][8]
-  int* header;         // [0] = slots in use
+  int* header;         // [0] = slots in use, [1], [2] = keys per piece
+  int* prefix;         // R > kWaveRequests: [2][R + 1] items and slots before each request
 };
 
 // 256 zero bytes: what rows that no query may see, and pages that do not exist, read as
@@ -192,6 +196,179 @@ __device__ __forceinline__ Request request(const PagedAttnArgs& a, const FastArg
   q.klo = a.window > 0 ? max(q.start + q.shift - a.window + 1, 0) : 0;
   if (q.khi < q.klo) q.khi = q.klo;
   return q;
+}
+
+// Work of a request in keys walked by a workgroup: a 64-key step of a chunk takes as long as a 128-key one of few rows.
+__device__ __forceinline__ float request_cost(const Request& q) {
+  return (float)q.tiles * (float)(q.khi - q.klo) * (q.chunk ? 2.f : 1.f);
+}
+struct PieceSize {
+  int few, chunk;      // keys
+};
+__device__ __forceinline__ PieceSize piece_size(float cost, int nkv, int target) {
+  const float budget = cost * (float)nkv / (float)target;
+  PieceSize p;
+  p.few = max((int)fminf(budget / (float)kFewStep, 8e6f) + 1, 2) * kFewStep;
+  p.chunk = max((int)fminf(budget * 0.5f / (float)kChunkStep, 8e6f) + 1, 8) * kChunkStep;
+  return p;
+}
+__device__ __forceinline__ int pieces(const Request& q, const PieceSize& p) {
+  const int len = q.khi - q.klo, step = q.chunk ? p.chunk : p.few;
+  return len <= step ? 1 : (len + step - 1) / step;
+}
+
+// Inclusive prefix sum over the wave by register moves between lanes (shifts inside rows of 16, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+__device__ __forceinline__ float wave_total(float x) {
+  auto dpp = [](float v, auto ctrl, auto rows) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+#define DPA_STEP(ctrl, rows) x += dpp(x, std::integral_constant<int, ctrl>(), std::integral_constant<int, rows>())
+  DPA_STEP(0x111, 0xf);
+  DPA_STEP(0x112, 0xf);
+  DPA_STEP(0x114, 0xf);
+  DPA_STEP(0x118, 0xf);
+  DPA_STEP(0x142, 0xa);
+  DPA_STEP(0x143, 0xc);
+#undef DPA_STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+struct Item {
+  int r, j, slot, np;      // request, number inside it, slot of its output, pieces of its keys; r < 0: none
+};
+// Item `id`, found by one wave; every wave of the grid comes to the same list.
+__device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs& f, int id, int lane) {
+  Item it;
+  it.r = -1;
+  if (a.R <= kWaveRequests) {
+    constexpr int PER = kWaveRequests / 64;      // consecutive requests per lane
+    Request q[PER];
+    float cost = 0.f;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      q[u].tiles = 0;
+      const int per = (a.R + 63) >> 6, r = lane * per + u;
+      if (u < per && r < a.R) {
+        q[u] = request(a, f, r);
+        cost += request_cost(q[u]);
+      }
+    }
+    const PieceSize size = piece_size(wave_total(cost), a.nkv, f.target);
+    int items[PER], slots[PER], ni = 0, ns = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      items[u] = slots[u] = 0;
+      if (q[u].tiles > 0) {
+        const int np = pieces(q[u], size);
+        items[u] = q[u].tiles * np * a.nkv;
+        slots[u] = np > 1 ? items[u] : 0;
+      }
+      ni += items[u];
+      ns += slots[u];
+    }
+    const int pi = wave_scan(ni), ps = wave_scan(ns);
+    if (id == 0 && lane == 63) f.header[0] = min(ps, f.max_slots);
+    const unsigned long long here = __ballot(id >= pi - ni && id < pi);
+    if (here == 0ull) return it;
+    const int src = __builtin_ctzll(here);
+    int first = pi - ni, slot = ps - ns, u = 0;
+    // the request of that lane
+#pragma unroll
+    for (int v = 0; v + 1 < PER; ++v)
+      if (u == v && id >= first + items[v]) {
+        first += items[v];
+        slot += slots[v];
+        u = v + 1;
+      }
+    int np = 1;
+#pragma unroll
+    for (int v = 0; v < PER; ++v)
+      if (u == v && q[v].tiles > 0) np = pieces(q[v], size);
+    it.r = src * ((a.R + 63) >> 6) + __builtin_amdgcn_readlane(u, src);
+    it.j = id - __builtin_amdgcn_readlane(first, src);
+    it.slot = __builtin_amdgcn_readlane(slot, src) + it.j;
+    it.np = __builtin_amdgcn_readlane(np, src);
+    return it;
+  }
+  // many requests: the prefixes lie in memory; 64 of them at a time
+  int lo = 0, n = a.R;       // the item belongs to a request in [lo, lo + n)
+  if (id >= f.prefix[a.R]) return it;
+  while (n > 1) {
+    const int per = (n + 63) >> 6, at = lo + lane * per;
+    const unsigned long long below = __ballot(lane * per < n && f.prefix[at] <= id);
+    if (below == 0ull) return it;
+    const int src = 63 - __builtin_clzll(below);
+    n = min(per, n - src * per);
+    lo += src * per;
+  }
+  it.r = lo;
+  it.j = id - f.prefix[lo];
+  it.slot = f.prefix[a.R + 1 + lo] + it.j;
+  const Request q = request(a, f, lo);
+  PieceSize size;
+  size.few = f.header[1];
+  size.chunk = f.header[2];
+  it.np = pieces(q, size);
+  return it;
+}
+
+// The prefixes for many requests: one workgroup.
+__global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a, FastArgs f) {
+  __shared__ float red_f[16];
+  __shared__ int red_i[16], red_s[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float cost = 0.f;
+  for (int r = tid; r < a.R; r += 1024) cost += request_cost(request(a, f, r));
+  cost = block_sum(cost, red_f);
+  const PieceSize size = piece_size(cost, a.nkv, f.target);
+  int base_i = 0, base_s = 0;
+  for (int r0 = 0; r0 < a.R; r0 += 1024) {
+    const int r = r0 + tid;
+    int ni = 0, ns = 0;
+    if (r < a.R) {
+      const Request q = request(a, f, r);
+      const int np = pieces(q, size);
+      ni = q.tiles * np * a.nkv;
+      ns = np > 1 ? ni : 0;
+    }
+    int pi = wave_scan(ni), ps = wave_scan(ns);
+    if (lane == 63) {
+      red_i[wave] = pi;
+      red_s[wave] = ps;
+    }
+    __syncthreads();
+    int ti = 0, ts = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w == wave) {
+        pi += ti;
+        ps += ts;
+      }
+      ti += red_i[w];
+      ts += red_s[w];
+    }
+    if (r < a.R) {
+      f.prefix[r] = base_i + pi - ni;
+      f.prefix[a.R + 1 + r] = base_s + ps - ns;
+    }
+    base_i += ti;
+    base_s += ts;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    f.prefix[a.R] = base_i;
+    f.header[0] = min(base_s, f.max_slots);
+    f.header[1] = size.few;
+    f.header[2] = size.chunk;
+  }
 }
 
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -228,16 +405,16 @@ struct PageRows {
   const int* table;       // the request's row
   unsigned long long kb, vb;
   int klo, khi, lane;
-  bool checked;           // every page of the range exists
+  bool gone;              // a page of the rows fetched last does not exist
   unsigned kv_off[2][VAR];
   int pg[NP];
 
-  __device__ __forceinline__ void init(const PagedAttnArgs& args, const int* t, int g, int lo, int hi, bool ok, int lane_) {
+  __device__ __forceinline__ void init(const PagedAttnArgs& args, const int* t, int g, int lo, int hi, int lane_) {
     a = &args;
     table = t;
     klo = lo;
     khi = hi;
-    checked = ok;
+    gone = false;
     lane = lane_;
     kb = (unsigned long long)args.k + 2ull * (unsigned long long)(g * args.k_hs);
     vb = (unsigned long long)args.v + 2ull * (unsigned long long)(g * args.v_hs);
@@ -249,28 +426,45 @@ struct PageRows {
       kv_off[1][v] = (unsigned)(lane / CPR) * (unsigned)(2 * args.v_rs) + col;
     }
   }
-  __device__ __forceinline__ bool whole(int ks0) const { return UNI && checked && ks0 >= klo && ks0 + NP * RPP <= khi; }
+  __device__ __forceinline__ bool whole(int ks0) const { return UNI && ks0 >= klo && ks0 + NP * RPP <= khi; }
   // page numbers of the rows [ks0, ks0 + NP * RPP), for the issue() of those rows
   __device__ __forceinline__ void fetch(int ks0) {
-    if (!whole(ks0)) return;
+    bool bad = false;
+    if (whole(ks0)) {
 #pragma unroll
-    for (int pc = 0; pc < NP; ++pc) {
-      const int col = fast_div(ks0 + pc * RPP, a->by_page);
-      typedef const __attribute__((address_space(4))) int* scalar_ptr;
-      pg[pc] = *(scalar_ptr)(unsigned long long)(table + __builtin_amdgcn_readfirstlane(col));
+      for (int pc = 0; pc < NP; ++pc) {
+        const int col = fast_div(ks0 + pc * RPP, a->by_page);
+        typedef const __attribute__((address_space(4))) int* scalar_ptr;
+        pg[pc] = *(scalar_ptr)(unsigned long long)(table + __builtin_amdgcn_readfirstlane(col));
+      }
+#pragma unroll
+      for (int pc = 0; pc < NP; ++pc) bad |= (unsigned)pg[pc] >= (unsigned)a->pages;
+    } else {
+#pragma unroll
+      for (int pc = 0; pc < NP; ++pc) {
+        const int key = ks0 + pc * RPP + lane / CPR;
+        pg[pc] = -1;
+        if (key >= klo && key < khi) {
+          pg[pc] = table[fast_div(key, a->by_page)];
+          bad |= (unsigned)pg[pc] >= (unsigned)a->pages;
+        }
+      }
+      bad = __any(bad);
     }
+    gone = bad;
   }
   template <bool V>
   __device__ __forceinline__ void issue(int ks0, unsigned lds) const {
     const unsigned long long base = V ? vb : kb;
     const unsigned long long ps = 2ull * (unsigned long long)(V ? a->v_ps : a->k_ps);
     const unsigned rs = 2u * (unsigned)(V ? a->v_rs : a->k_rs);
-    if (whole(ks0)) {
+    if (whole(ks0) && !gone) {
 #pragma unroll
       for (int pc = 0; pc < NP; ++pc) {
         const int key = ks0 + pc * RPP;
         const int row = __builtin_amdgcn_readfirstlane(key - fast_div(key, a->by_page) * a->page);
-        dma_uniform(base + (unsigned)pg[pc] * ps + (unsigned)row * rs, kv_off[V][pc % VAR], lds + pc * 1024);
+        const unsigned p = __builtin_amdgcn_readfirstlane(pg[pc]);
+        dma_uniform(base + p * ps + (unsigned)row * rs, kv_off[V][pc % VAR], lds + pc * 1024);
       }
       return;
     }
@@ -279,12 +473,9 @@ struct PageRows {
       const int row = pc * RPP + lane / CPR, key = ks0 + row;
       const int ch = swz<W>(row, lane % CPR);
       unsigned long long addr = (unsigned long long)zero_row + 16u * ch;
-      if (key >= klo && key < khi) {
-        const int col = fast_div(key, a->by_page);
-        const int p = table[col];
-        if (p >= 0 && p < a->pages && ch * 8 < a->width)
-          addr = base + (unsigned)p * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
-      }
+      const int col = fast_div(max(key, 0), a->by_page);
+      if ((unsigned)pg[pc] < (unsigned)a->pages && key >= klo && key < khi && ch * 8 < a->width)
+        addr = base + (unsigned)pg[pc] * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
       dma_lane(addr, lds + pc * 1024);
     }
   }
@@ -456,13 +647,11 @@ __device__ __forceinline__ float* o_piece(char* tile, int row, int piece) {
   return reinterpret_cast<float*>(tile + row * (W * 4) + 16 * (piece ^ (row & (W / 4 - 1))));
 }
 
-template <typename T, int W, bool UNI>
-__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
+template <typename T, int W, bool UNI, bool CHUNKS>
+__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
   constexpr int NK = W / 16, ND = W / 32, SUB = 32 * W * 2, REGION = 4 * SUB / 2;   // REGION: a wave's 32 x W fp32 = 2 SUB
   static_assert(REGION == 2 * SUB, "one K and one V subtile per wave");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red_f[4];
-  __shared__ int red_i[4], red_s[4], found[8];
   __shared__ float ml_s[4][32][2];
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -482,76 +671,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
   }
 
   // ---- this workgroup's item ----
-  const int per = (a.R + kThreads - 1) / kThreads;      // consecutive requests per thread
-  const int ra = min(tid * per, a.R), rb = min(ra + per, a.R);
-  float cost = 0.f;
-  for (int r = ra; r < rb; ++r) {
-    const Request q = request(a, f, r);
-    cost += (float)q.tiles * (float)(q.khi - q.klo) * (q.chunk ? 2.f : 1.f);
-  }
-  cost = wave_sum(cost);
-  if (lane == 0) red_f[wave] = cost;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  const float budget = (red_f[0] + red_f[1] + red_f[2] + red_f[3]) * (float)a.nkv / (float)f.target;
-  const int few_keys = max((int)fminf(budget / (float)kFewStep, 8e6f) + 1, 2) * kFewStep;
-  const int chunk_keys = max((int)fminf(budget * 0.5f / (float)kChunkStep, 8e6f) + 1, 8) * kChunkStep;
-  auto pieces = [&](const Request& q) {
-    const int len = q.khi - q.klo, step = q.chunk ? chunk_keys : few_keys;
-    return len <= step ? 1 : (len + step - 1) / step;
-  };
-  int items = 0, slots = 0;
-  for (int r = ra; r < rb; ++r) {
-    const Request q = request(a, f, r);
-    const int np = pieces(q), k = q.tiles * np * a.nkv;
-    items += k;
-    if (np > 1) slots += k;
-  }
-  int pi = items, ps = slots;     // inclusive prefixes over the threads
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int x = __shfl_up(pi, off, 64), y = __shfl_up(ps, off, 64);
-    if (lane >= off) {
-      pi += x;
-      ps += y;
-    }
-  }
-  if (lane == 63) {
-    red_i[wave] = pi;
-    red_s[wave] = ps;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w)
-    if (w < wave) {
-      pi += red_i[w];
-      ps += red_s[w];
-    }
-  pi -= items;
-  ps -= slots;
-  const int id = blockIdx.x;
-  if (id == 0 && tid == kThreads - 1 && f.header != nullptr) f.header[0] = min(ps + slots, f.max_slots);
-  if (id >= pi && id < pi + items) {
-    for (int r = ra; r < rb; ++r) {
-      const Request q = request(a, f, r);
-      const int np = pieces(q), k = q.tiles * np * a.nkv;
-      if (id < pi + k) {
-        found[0] = r;
-        found[1] = id - pi;
-        found[2] = ps + id - pi;
-        found[3] = np;
-        break;
-      }
-      pi += k;
-      if (np > 1) ps += k;
-    }
-  }
-  __syncthreads();
-  const int r = __builtin_amdgcn_readfirstlane(found[0]);
+  const Item it = find_item(a, f, blockIdx.x, lane);
+  const int r = __builtin_amdgcn_readfirstlane(it.r);
   if (r < 0) return;
-  const Request q = request(a, f, r);
-  const int np = __builtin_amdgcn_readfirstlane(found[3]), slot = __builtin_amdgcn_readfirstlane(found[2]);
-  int j = __builtin_amdgcn_readfirstlane(found[1]);
+  Request q = request(a, f, r);
+  if (!CHUNKS) q.chunk = false;      // the host has ruled them out: the compiler may too
+  const int np = __builtin_amdgcn_readfirstlane(it.np), slot = __builtin_amdgcn_readfirstlane(it.slot);
+  int j = __builtin_amdgcn_readfirstlane(it.j);
   const int g = j % a.nkv;
   j /= a.nkv;
   const int piece = j % np;
@@ -566,14 +692,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
   const int span = ((khi - k_base + np - 1) / np + step - 1) / step * step;
   const int k0 = k_base + piece * span, k1 = min(khi, k0 + span);
 
-  // ---- do all pages of the piece exist? ----
+  // ---- chunks: do all pages of the piece exist? (few rows look at every subtile's) ----
   const int* table = a.table + (long long)r * a.table_ld;
   bool missing = false;
-  if (k1 > k0) {
+  if (q.chunk && k1 > k0) {
     const int c_lo = fast_div(max(k0, klo), a.by_page), c_hi = fast_div(k1 - 1, a.by_page);
     for (int col = c_lo + tid; col <= c_hi; col += kThreads) missing |= (unsigned)table[col] >= (unsigned)a.pages;
   }
-  missing = __syncthreads_or(missing);
+  if (q.chunk) missing = __syncthreads_or(missing);
 
   // ---- queries of this lane's row ----
   const int row = rows0 + (q.chunk ? wave * 32 : 0) + r32;
@@ -602,9 +728,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
     st.hi = valid ? min(pos, cap - 1) : -1;
     st.lo = a.window > 0 ? pos - a.window + 1 : 0;
   }
-  auto hide_missing = [&](int ks0) {
+  auto hide_missing = [&](int ks0, bool gone_pages) {
     return [=](f32x16& s) {
-      if (!missing) return;
+      if (!gone_pages) return;
 #pragma unroll 1
       for (int i = 0; i < 32; ++i) {     // one page number at a time, the same for all lanes
         const int key = ks0 + i;
@@ -626,7 +752,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
     char* const vt = kt + SUB;
     const unsigned k_lds = lds0 + wave * REGION, v_lds = k_lds + SUB;
     PageRows<W, NP, UNI> pr;
-    pr.init(a, table, g, klo, khi, !missing, lane);
+    pr.init(a, table, g, klo, khi, lane);
     int ks0 = k0 + wave * 32;
     if (ks0 < k1) {
       pr.fetch(ks0);
@@ -636,7 +762,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
     for (; ks0 < k1; ks0 += 128) {
       const int next = ks0 + 128;
       const bool more = next < k1;
-      const bool mask = missing || ks0 + 31 > p_first || ks0 + 32 > cap || (a.window > 0 && ks0 < p_last - a.window + 1);
+      const bool gone = pr.gone;
+      const bool mask = gone || ks0 + 31 > p_first || ks0 + 32 > cap || (a.window > 0 && ks0 < p_last - a.window + 1);
       if (more) pr.fetch(next);
       wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
       subtile<T, W>(
@@ -653,7 +780,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
             wait_lds();
             if (more) pr.template issue<true>(next, v_lds);
           },
-          hide_missing(ks0));
+          hide_missing(ks0, gone));
     }
     // ---- merge the waves ----
     const float l = sum_halves(st.l);
@@ -722,7 +849,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
     // ---- chunks: the waves share 64-key tiles ----
     constexpr int NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;    // pieces per wave; K and V tile
     PageRows<W, NP, UNI> pr;
-    pr.init(a, table, g, klo, khi, !missing, lane);
+    pr.init(a, table, g, klo, khi, lane);
     constexpr int WROWS = 16;       // rows of a tile that a wave transfers
     const int w_off = wave * WROWS;
     const unsigned w_lds = lds0 + wave * NP * 1024;
@@ -757,7 +884,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
         if (ks0 > wp_last || ks0 >= khi) break;
         if (a.window > 0 && ks0 + 31 < wp_first - a.window + 1) continue;
         const bool mask = missing || ks0 + 31 > wp_first || ks0 + 32 > cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
-        subtile<T, W>(kt + sub * SUB, vt + sub * SUB, ks0, mask, f.c, qf, st, lane, [] {}, [] {}, [] {}, hide_missing(ks0));
+        subtile<T, W>(kt + sub * SUB, vt + sub * SUB, ks0, mask, f.c, qf, st, lane, [] {}, [] {}, [] {}, hide_missing(ks0, missing));
       }
     }
     const float l = sum_halves(st.l);
@@ -805,42 +932,78 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
   }
 }
 
-// The pieces of one row tile and KV head: o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, in the order of the keys.
+// The pieces of one row tile and KV head: o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p. A workgroup takes kJoinRows
+// rows; a thread has 8 columns of a row and every `groups`-th piece, four of them requested together, and the groups are
+// joined through LDS: always in the same order.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs a, FastArgs f) {
+  constexpr int CPR = W / 8, kJoinRows = kThreads / CPR, U = 4;
+  __shared__ float o_s[kThreads][9], m_s[kThreads];      // (9: rows of 8 floats would share banks)
   const int slot = blockIdx.x;
   if (slot >= f.header[0]) return;
-  const int* m = f.meta + (long long)slot * 8;
-  const int np = m[0], start = m[1], rows0 = m[2], nrows = m[3], g = m[4];
-  if (np < 2) return;
-  for (int i = threadIdx.x; i < nrows * (W / 8); i += kThreads) {
-    const int rr = i / (W / 8), d8 = i % (W / 8);
-    if (8 * d8 >= a.width) continue;
-    float M = -INFINITY, L = 0.f, o[8];
+  const int* meta = f.meta + (long long)slot * 8;
+  const int np = meta[0], start = meta[1], rows0 = meta[2], nrows = min(meta[3] - (int)blockIdx.y * kJoinRows, kJoinRows), g = meta[4];
+  if (np < 2 || nrows <= 0) return;
+  const int row_b = blockIdx.y * kJoinRows, units = nrows * CPR;
+  int groups = 1;
+  while (2 * groups * units <= kThreads) groups *= 2;
+  const int tid = threadIdx.x, unit = tid % units, grp = tid / units;
+  const int rr = row_b + unit / CPR, d8 = unit % CPR;
+  float M = -INFINITY, L = 0.f, o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    for (int p = 0; p < np; ++p) {
-      const float* ml = f.ml + ((long long)(slot + p * a.nkv) * f.slot_rows + rr) * 2;
-      if (ml[1] != 0.f) M = fmaxf(M, ml[0]);
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  if (grp < groups) {
+    for (int p0 = grp; p0 < np; p0 += groups * U) {
+      float m[U], l[U], x[U][8];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int p = min(p0 + u * groups, np - 1);
+        const long long at = (long long)(slot + p * a.nkv) * f.slot_rows + rr;
+        m[u] = f.ml[at * 2];
+        l[u] = p0 + u * groups < np ? f.ml[at * 2 + 1] : 0.f;
+        load8(f.part + at * W + 8 * d8, x[u]);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (l[u] != 0.f) top = fmaxf(top, m[u]);
+      const float keep = L != 0.f ? __builtin_amdgcn_exp2f(M - top) : 0.f;
+      L *= keep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (l[u] != 0.f) {
+          const float w = __builtin_amdgcn_exp2f(m[u] - top);
+          L += l[u] * w;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] += x[u][e] * w;
+        }
+      M = top;
     }
-    for (int p = 0; p < np; ++p) {
-      const long long at = (long long)(slot + p * a.nkv) * f.slot_rows + rr;
-      const float l = f.ml[at * 2 + 1];
-      if (l == 0.f) continue;
-      const float w = __builtin_amdgcn_exp2f(f.ml[at * 2] - M);
-      float x[8];
-      load8(f.part + at * W + 8 * d8, x);
-      L += l * w;
+    m_s[tid] = M;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] += x[e] * w;
-    }
-    const float inv = L != 0.f ? 1.f / L : 0.f;
-    u32x4 w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = L != 0.f ? Frag<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
-    const int tk = fast_div(rows0 + rr, f.by_group), hd = g * f.G + rows0 + rr - tk * f.G;
-    *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
+    for (int e = 0; e < 8; ++e) o_s[tid][e] = o[e];
+    o_s[tid][8] = L;
   }
+  __syncthreads();
+  if (grp != 0 || 8 * d8 >= a.width) return;
+  for (int w = 1; w < groups; ++w) {
+    const int t = unit + w * units;
+    const float m = m_s[t], l = o_s[t][8];
+    if (l == 0.f) continue;
+    const float top = fmaxf(M, m), keep = L != 0.f ? __builtin_amdgcn_exp2f(M - top) : 0.f, add = __builtin_amdgcn_exp2f(m - top);
+    L = L * keep + l * add;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = o[e] * keep + o_s[t][e] * add;
+    M = top;
+  }
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = L != 0.f ? Frag<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
+  const int tk = fast_div(rows0 + rr, f.by_group), hd = g * f.G + rows0 + rr - tk * f.G;
+  *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
 }
 
 // Whether the matrix kernels take the call: 16-bit types, whole aligned 16-byte pieces, offsets inside a page below 2^32.
@@ -857,46 +1020,49 @@ bool fast_ok(const PagedAttnArgs& a) {
 
 struct Plan {
   int target, grid, slots, slot_rows;
+  bool chunks;
   size_t part, ml, meta, total;
 };
 Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   Plan p;
   const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
+  p.chunks = (long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows;
   p.target = num_cus * 4;
+  if (const char* e = getenv("PA_TARGET")) p.target = atoi(e);
   // tiles: one per request with rows, and one more for every 128 rows of a chunk
   const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
   p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
   p.slots = (int)std::min<long long>(2ll * p.target, p.grid);
-  p.slot_rows = (long long)a.N * G > kFewRows ? kChunkRows : kFewRows;
+  p.slot_rows = p.chunks ? kChunkRows : kFewRows;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.part = up((size_t)p.slots * p.slot_rows * W * 4);
   p.ml = up((size_t)p.slots * p.slot_rows * 8);
   p.meta = up((size_t)p.slots * 32);
-  p.total = p.part + p.ml + p.meta + 256;
+  p.total = p.part + p.ml + p.meta + 256 + (a.R > kWaveRequests ? up((size_t)(a.R + 1) * 8) : 0);
   return p;
 }
 
-template <typename T, int W, bool UNI>
+template <typename T, int W, bool UNI, bool CHUNKS>
 void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
   constexpr int lds = 4 * 2 * 32 * W * 2;
   static bool set = false;       // above the default limit of dynamic LDS; the same value every time
   if (!set) {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, W, UNI>),
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, W, UNI, CHUNKS>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     set = true;
   }
-  hipLaunchKernelGGL((paged_attn_kernel<T, W, UNI>), dim3(grid), dim3(kThreads), lds, st, a, f);
-  if (f.max_slots > 0) hipLaunchKernelGGL((paged_attn_join_kernel<T, W>), dim3(f.max_slots), dim3(kThreads), 0, st, a, f);
+  if (a.R > kWaveRequests) hipLaunchKernelGGL(paged_attn_items_kernel, dim3(1), dim3(1024), 0, st, a, f);
+  hipLaunchKernelGGL((paged_attn_kernel<T, W, UNI, CHUNKS>), dim3(grid), dim3(kThreads), lds, st, a, f);
+  hipLaunchKernelGGL((paged_attn_join_kernel<T, W>), dim3(f.max_slots, (f.slot_rows * (W / 8) + kThreads - 1) / kThreads),
+                     dim3(kThreads), 0, st, a, f);
 }
-template <typename T>
-void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
-  if (a.width <= 64) {
-    if (a.width == 64 && a.page % 8 == 0) launch_fast<T, 64, true>(a, f, grid, st);
-    else launch_fast<T, 64, false>(a, f, grid, st);
-  } else {
-    if (a.width == 128 && a.page % 4 == 0) launch_fast<T, 128, true>(a, f, grid, st);
-    else launch_fast<T, 128, false>(a, f, grid, st);
-  }
+template <typename T, int W>
+void launch_fast(const PagedAttnArgs& a, const FastArgs& f, const Plan& p, hipStream_t st) {
+  const bool uni = a.width == W && a.page % (512 / W) == 0;      // a 1 KiB transfer lies in one page
+  if (uni && p.chunks) launch_fast<T, W, true, true>(a, f, p.grid, st);
+  else if (uni) launch_fast<T, W, true, false>(a, f, p.grid, st);
+  else if (p.chunks) launch_fast<T, W, false, true>(a, f, p.grid, st);
+  else launch_fast<T, W, false, false>(a, f, p.grid, st);
 }
 
 }  // namespace
@@ -915,7 +1081,6 @@ void paged_attn(const PagedAttnArgs& a, int num_cus, void* workspace, hipStream_
     f.G = a.nh / a.nkv;
     f.by_group = make_fast_div(f.G);
     f.target = p.target;
-    f.max_items = p.grid;
     f.max_slots = p.slots;
     f.slot_rows = p.slot_rows;
     char* w = (char*)workspace;
@@ -923,8 +1088,10 @@ void paged_attn(const PagedAttnArgs& a, int num_cus, void* workspace, hipStream_
     f.ml = (float*)(w + p.part);
     f.meta = (int*)(w + p.part + p.ml);
     f.header = (int*)(w + p.part + p.ml + p.meta);
-    if (a.type == kTypeBf16) launch_fast<bf16_t>(a, f, p.grid, st);
-    else launch_fast<half_t>(a, f, p.grid, st);
+    f.prefix = f.header + 64;
+    const bool bf = a.type == kTypeBf16;
+    if (a.width <= 64) bf ? launch_fast<bf16_t, 64>(a, f, p, st) : launch_fast<half_t, 64>(a, f, p, st);
+    else bf ? launch_fast<bf16_t, 128>(a, f, p, st) : launch_fast<half_t, 128>(a, f, p, st);
     return;
   }
   const long long waves = (long long)a.N * a.nh;

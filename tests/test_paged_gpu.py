@@ -184,6 +184,16 @@ def test_attention_long_contexts(qn, ctx, width):
     check_attention(qn, ctx, 8, 2, width, 16, BF)
 
 
+@pytest.mark.parametrize("R", [63, 64, 65, 255, 256, 257, 1100, 4200])
+@pytest.mark.parametrize("chunks", [False, True])
+def test_attention_many_requests(R, chunks):
+    rng = random.Random(R)
+    qn = [1 if rng.random() < 0.9 else rng.choice([0, 2, 40 if chunks else 3]) for _ in range(R)]
+    ctx = [rng.choice([0, 3, 20, 40]) for _ in range(R)]
+    ctx[R // 3] = 3000
+    check_attention(qn, ctx, 4, 2, 64, 16, BF, max_q=None if chunks else 3)
+
+
 @pytest.mark.parametrize("dtype,width", [(FP, 64), (FP, 100), (BF, 20), (HF, 7), (BF, 200), (BF, 256), (FP, 1)])
 def test_attention_other_types_and_widths(dtype, width):
     check_attention([1, 40, 0, 2], [100, 33, 0, 0], 4, 2, width, 16, dtype, pad=1)
