@@ -181,6 +181,10 @@ struct Request {
   int klo, khi;        // keys that any of its rows sees
   bool chunk;
 };
+__device__ __forceinline__ void key_range(const PagedAttnArgs& a, Request& q) {
+  q.klo = a.window > 0 ? max(q.start + q.shift - a.window + 1, 0) : 0;
+  q.khi = max(min(q.start + q.n + q.shift, a.M * a.page), q.klo);
+}
 __device__ __forceinline__ Request request(const PagedAttnArgs& a, const FastArgs& f, int r) {
   Request q;
   const int c0 = a.cu_q[r], c1 = a.cu_q[r + 1];
@@ -191,10 +195,7 @@ __device__ __forceinline__ Request request(const PagedAttnArgs& a, const FastArg
   q.rows = q.n * f.G;
   q.chunk = q.rows > kFewRows;
   q.tiles = q.chunk ? (q.rows + kChunkRows - 1) / kChunkRows : (q.rows > 0 ? 1 : 0);
-  const int cap = a.M * a.page;
-  q.khi = min(q.start + q.n + q.shift, cap);
-  q.klo = a.window > 0 ? max(q.start + q.shift - a.window + 1, 0) : 0;
-  if (q.khi < q.klo) q.khi = q.klo;
+  key_range(a, q);
   return q;
 }
 
@@ -240,6 +241,21 @@ __device__ __forceinline__ float wave_total(float x) {
   DPA_STEP(0x143, 0xc);
 #undef DPA_STEP
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// Many requests, whose prefixes lie in memory: the last r with prefix[r] <= x < prefix[R], 64 of them at a time.
+__device__ __forceinline__ int find_prefix(const int* prefix, int R, int x, int lane) {
+  int lo = 0, n = R;
+  if (x >= prefix[R]) return -1;
+  while (n > 1) {
+    const int per = (n + 63) >> 6, at = lo + lane * per;
+    const unsigned long long below = __ballot(lane * per < n && prefix[at] <= x);
+    if (below == 0ull) return -1;
+    const int src = 63 - __builtin_clzll(below);
+    n = min(per, n - src * per);
+    lo += src * per;
+  }
+  return lo;
 }
 
 struct Item {
@@ -299,17 +315,8 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
     it.np = __builtin_amdgcn_readlane(np, src);
     return it;
   }
-  // many requests: the prefixes lie in memory; 64 of them at a time
-  int lo = 0, n = a.R;       // the item belongs to a request in [lo, lo + n)
-  if (id >= f.prefix[a.R]) return it;
-  while (n > 1) {
-    const int per = (n + 63) >> 6, at = lo + lane * per;
-    const unsigned long long below = __ballot(lane * per < n && f.prefix[at] <= id);
-    if (below == 0ull) return it;
-    const int src = 63 - __builtin_clzll(below);
-    n = min(per, n - src * per);
-    lo += src * per;
-  }
+  const int lo = find_prefix(f.prefix, a.R, id, lane);
+  if (lo < 0) return it;
   it.r = lo;
   it.j = id - f.prefix[lo];
   it.slot = f.prefix[a.R + 1 + lo] + it.j;
@@ -321,14 +328,82 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
   return it;
 }
 
+// ---- few rows only: equal shares of all steps ----
+// A (request, 32 packed rows, KV head) is a run of 128-key steps (one at least); the runs lie one after another, and workgroup i of `eff`
+// takes steps [i * per, (i + 1) * per) of them all, whichever runs they fall into: contexts of any mix of lengths load
+// the card evenly in one round. At most its first and its last run are cut.
+constexpr int kMinSteps = 2;           // fewer steps than this are not worth a workgroup of their own
+__device__ __forceinline__ int run_base(const Request& q) { return q.klo & ~31; }
+__device__ __forceinline__ int run_steps(const Request& q) {
+  return q.rows > 0 ? max((q.khi - run_base(q) + kFewStep - 1) / kFewStep, 1) : 0;
+}
+__device__ __forceinline__ int run_count(const Request& q, int nkv) { return (q.rows + kFewRows - 1) / kFewRows * nkv; }
+
+struct Runs {        // the requests of the batch in LDS (R <= kWaveRequests)
+  int before[kWaveRequests + 1];       // steps before each
+  int start[kWaveRequests], rows[kWaveRequests], shift[kWaveRequests];
+  int red[kThreads / 64];
+};
+static_assert(kWaveRequests == kThreads, "one request per thread");
+// Steps of all runs; leaves `runs` filled for every thread.
+__device__ __forceinline__ int list_runs(const PagedAttnArgs& a, const FastArgs& f, Runs& runs) {
+  if (a.R > kWaveRequests) return f.prefix[a.R];
+  const int tid = threadIdx.x;
+  int steps = 0;
+  if (tid < a.R) {
+    const Request q = request(a, f, tid);
+    steps = run_steps(q) * run_count(q, a.nkv);
+    runs.start[tid] = q.start;
+    runs.rows[tid] = q.rows;
+    runs.shift[tid] = q.shift;
+  }
+  int incl = wave_scan(steps);
+  if (a.R > 64) {
+    if ((tid & 63) == 63) runs.red[tid >> 6] = incl;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64 - 1; ++w)
+      if (w < (tid >> 6)) incl += runs.red[w];
+  }
+  if (tid < a.R) runs.before[tid + 1] = incl;
+  if (tid == 0) runs.before[0] = 0;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(runs.before[a.R]);
+}
+// The request of step `at`, and the number of its first step; r < 0: there is none.
+__device__ __forceinline__ int find_run(const PagedAttnArgs& a, const FastArgs& f, const Runs& runs, int at, int& first, Request& q) {
+  const int lane = threadIdx.x & 63;
+  if (a.R > kWaveRequests) {
+    const int r = find_prefix(f.prefix, a.R, at, lane);
+    if (r < 0) return -1;
+    first = __builtin_amdgcn_readfirstlane(f.prefix[r]);
+    q = request(a, f, r);
+    return r;
+  }
+  int below = 0;
+  for (int u = 0; u < a.R; u += 64) below += __popcll(__ballot(u + lane < a.R && runs.before[u + lane] <= at));
+  const int r = below - 1;
+  if (r < 0) return -1;
+  first = __builtin_amdgcn_readfirstlane(runs.before[r]);
+  q.start = __builtin_amdgcn_readfirstlane(runs.start[r]);
+  q.rows = __builtin_amdgcn_readfirstlane(runs.rows[r]);
+  q.shift = __builtin_amdgcn_readfirstlane(runs.shift[r]);
+  q.n = fast_div(q.rows, f.by_group);
+  key_range(a, q);
+  return r;
+}
+
 // The prefixes for many requests: one workgroup.
+template <bool CHUNKS>
 __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a, FastArgs f) {
   __shared__ float red_f[16];
   __shared__ int red_i[16], red_s[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float cost = 0.f;
-  for (int r = tid; r < a.R; r += 1024) cost += request_cost(request(a, f, r));
-  cost = block_sum(cost, red_f);
+  if (CHUNKS) {
+    for (int r = tid; r < a.R; r += 1024) cost += request_cost(request(a, f, r));
+    cost = block_sum(cost, red_f);
+  }
   const PieceSize size = piece_size(cost, a.nkv, f.target);
   int base_i = 0, base_s = 0;
   for (int r0 = 0; r0 < a.R; r0 += 1024) {
@@ -336,8 +411,8 @@ __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a,
     int ni = 0, ns = 0;
     if (r < a.R) {
       const Request q = request(a, f, r);
-      const int np = pieces(q, size);
-      ni = q.tiles * np * a.nkv;
+      const int np = CHUNKS ? pieces(q, size) : 1;
+      ni = CHUNKS ? q.tiles * np * a.nkv : run_steps(q) * run_count(q, a.nkv);
       ns = np > 1 ? ni : 0;
     }
     int pi = wave_scan(ni), ps = wave_scan(ns);
@@ -365,7 +440,7 @@ __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a,
   }
   if (tid == 0) {
     f.prefix[a.R] = base_i;
-    f.header[0] = min(base_s, f.max_slots);
+    if (CHUNKS) f.header[0] = min(base_s, f.max_slots);
     f.header[1] = size.few;
     f.header[2] = size.chunk;
   }
@@ -518,18 +593,18 @@ template <typename T, int W>
 __device__ __forceinline__ void place_non_finite(u32x4 (&vf)[2][W / 32], f32x16 (&o)[W / 32], int lo_rel, int hi_rel, int hh) {
   typedef Frag<T> F;
   u32x4 seen[2];
+  const unsigned span = (unsigned)(hi_rel - lo_rel);     // hi_rel < lo_rel: no key, and no difference below reaches it
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      unsigned w = 0u;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int key = acc_row(8 * s2 + 2 * j + e, hh);
-        if (key >= lo_rel && key <= hi_rel) w |= F::kOne << (16 * e);
-      }
-      seen[s2][j] = w;
+      const unsigned k0 = (unsigned)(acc_row(8 * s2 + 2 * j, hh) - lo_rel);
+      seen[s2][j] = hi_rel < lo_rel ? 0u : (k0 <= span ? F::kOne : 0u) | (k0 + 1u <= span ? F::kOne << 16 : 0u);
     }
+  // one 16-bit value: code, and whether it stays
+  auto code_of = [](unsigned x) {
+    return (x & F::kInf) != F::kInf ? 0u : (x & 0x7fffu) != F::kInf ? F::k4096 : (x & F::kSign) ? F::k64 : F::kOne;
+  };
 #pragma unroll
   for (int dt = 0; dt < W / 32; ++dt) {
     f32x16 code;
@@ -540,27 +615,18 @@ __device__ __forceinline__ void place_non_finite(u32x4 (&vf)[2][W / 32], f32x16 
       u32x4 cw;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        unsigned w = vf[s2][dt][j], keep = w, c = 0u;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const unsigned x = (w >> (16 * e)) & 0xffffu;
-          if ((x & F::kInf) == F::kInf) {
-            keep &= ~(0xffffu << (16 * e));
-            c |= ((x & 0x7fffu) != F::kInf ? F::k4096 : (x & F::kSign) ? F::k64 : F::kOne) << (16 * e);
-          }
-        }
-        vf[s2][dt][j] = keep;
-        cw[j] = c;
+        const unsigned w = vf[s2][dt][j], lo = code_of(w & 0xffffu), hi = code_of(w >> 16);
+        vf[s2][dt][j] = (lo ? 0u : w & 0xffffu) | (hi ? 0u : w & 0xffff0000u);
+        cw[j] = lo | hi << 16;
       }
       code = F::mfma(cw, seen[s2], code);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int n = (int)code[i];
-      if (n != 0) {
-        const bool pos = (n & 63) != 0, neg = (n & 4032) != 0;
-        o[dt][i] += n >= 4096 || (pos && neg) ? __builtin_nanf("") : (pos ? INFINITY : -INFINITY);
-      }
+      const int n = (int)code[i], pos = n & 63, neg = n & 4032;
+      const float one_sign = pos ? INFINITY : -INFINITY;
+      const float what = n >= 4096 || (pos && neg) ? __builtin_nanf("") : one_sign;
+      o[dt][i] += n != 0 ? what : 0.f;
     }
   }
 }
@@ -647,288 +713,374 @@ __device__ __forceinline__ float* o_piece(char* tile, int row, int piece) {
   return reinterpret_cast<float*>(tile + row * (W * 4) + 16 * (piece ^ (row & (W / 4 - 1))));
 }
 
-template <typename T, int W, bool UNI, bool CHUNKS>
-__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
-  constexpr int NK = W / 16, ND = W / 32, SUB = 32 * W * 2, REGION = 4 * SUB / 2;   // REGION: a wave's 32 x W fp32 = 2 SUB
-  static_assert(REGION == 2 * SUB, "one K and one V subtile per wave");
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float ml_s[4][32][2];
-  const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
-
-  // ---- rows outside every sequence ----
-  if (a.zero_rest) {
-    const int lo = a.R > 0 ? min(max(a.cu_q[0], 0), a.N) : a.N, hi = a.R > 0 ? min(max(a.cu_q[a.R], 0), a.N) : a.N;
-    const int rest = lo + a.N - max(hi, lo);
-    const long long total = (long long)rest * a.nh * a.width;
-    for (long long i = (long long)blockIdx.x * kThreads + tid; i < total; i += (long long)gridDim.x * kThreads) {
-      const int d = (int)(i % a.width), h = (int)((i / a.width) % a.nh);
-      int row = (int)(i / a.width / a.nh);
-      if (row >= lo) row += max(hi, lo) - lo;
-      ((uint16_t*)a.o)[(long long)row * a.o_ts + (long long)h * a.o_hs + d] = 0;
-    }
-  }
-
-  // ---- this workgroup's item ----
-  const Item it = find_item(a, f, blockIdx.x, lane);
-  const int r = __builtin_amdgcn_readfirstlane(it.r);
-  if (r < 0) return;
-  Request q = request(a, f, r);
-  if (!CHUNKS) q.chunk = false;      // the host has ruled them out: the compiler may too
-  const int np = __builtin_amdgcn_readfirstlane(it.np), slot = __builtin_amdgcn_readfirstlane(it.slot);
-  int j = __builtin_amdgcn_readfirstlane(it.j);
-  const int g = j % a.nkv;
-  j /= a.nkv;
-  const int piece = j % np;
-  const int tile = q.tiles - 1 - j / np;                 // the rows that see most come first
-  if (tile < 0 || j < 0 || (np > 1 && (unsigned)slot >= (unsigned)f.max_slots)) return;   // lengths that contradict each other
-  const int rows0 = tile * kChunkRows, nrows = min(q.chunk ? kChunkRows : kFewRows, q.rows - rows0);
-  const int t_first = fast_div(rows0, f.by_group), t_last = fast_div(rows0 + nrows - 1, f.by_group);
-  const int p_first = q.start + t_first + q.shift, p_last = q.start + t_last + q.shift, cap = a.M * a.page;
-  const int khi = max(min(p_last + 1, cap), 0), klo = min(a.window > 0 ? max(p_first - a.window + 1, 0) : 0, khi);
-  const int step = q.chunk ? kChunkStep : kFewStep;
-  const int k_base = klo & ~63;
-  const int span = ((khi - k_base + np - 1) / np + step - 1) / step * step;
-  const int k0 = k_base + piece * span, k1 = min(khi, k0 + span);
-
-  // ---- chunks: do all pages of the piece exist? (few rows look at every subtile's) ----
-  const int* table = a.table + (long long)r * a.table_ld;
-  bool missing = false;
-  if (q.chunk && k1 > k0) {
-    const int c_lo = fast_div(max(k0, klo), a.by_page), c_hi = fast_div(k1 - 1, a.by_page);
-    for (int col = c_lo + tid; col <= c_hi; col += kThreads) missing |= (unsigned)table[col] >= (unsigned)a.pages;
-  }
-  if (q.chunk) missing = __syncthreads_or(missing);
-
-  // ---- queries of this lane's row ----
-  const int row = rows0 + (q.chunk ? wave * 32 : 0) + r32;
-  const bool valid = row < q.rows && (q.chunk || r32 < nrows);
-  const int tok = fast_div(valid ? row : 0, f.by_group), head = g * f.G + (valid ? row - tok * f.G : 0);
-  u32x4 qf[NK];
-  {
-    const uint16_t* qp = (const uint16_t*)a.q + (long long)(q.start + tok) * a.q_ts + (long long)head * a.q_hs;
-    const unsigned flip = f.negate ? 0x80008000u : 0u;
-#pragma unroll
-    for (int ks = 0; ks < NK; ++ks) {
-      const int d = ks * 16 + hh * 8;
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (valid && d < a.width) {
-        v = *reinterpret_cast<const u32x4*>(qp + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] ^= flip;
-      }
-      qf[ks] = v;
-    }
-  }
-  RowState<W> st;
+// A tile of packed rows of one request and KV head.
+struct Tile {
+  int start, shift, rows, rows0, nrows, g;
+  int p_first, p_last, klo, khi, cap;      // positions of its first and last row, keys that any of them sees
+  const int* table;
+};
+__device__ __forceinline__ Tile make_tile(const PagedAttnArgs& a, const FastArgs& f, const Request& q, int r, int g, int rows0,
+                                          int most) {
+  Tile t;
+  t.start = q.start;
+  t.shift = q.shift;
+  t.rows = q.rows;
+  t.rows0 = rows0;
+  t.nrows = min(most, q.rows - rows0);
+  t.g = g;
+  t.p_first = q.start + fast_div(rows0, f.by_group) + q.shift;
+  t.p_last = q.start + fast_div(rows0 + t.nrows - 1, f.by_group) + q.shift;
+  t.cap = a.M * a.page;
+  t.khi = max(min(t.p_last + 1, t.cap), 0);
+  t.klo = min(a.window > 0 ? max(t.p_first - a.window + 1, 0) : 0, t.khi);
+  t.table = a.table + (long long)r * a.table_ld;
+  return t;
+}
+// Packed row i of the tile's request: row of the batch and head.
+__device__ __forceinline__ long long row_offset(const FastArgs& f, const Tile& t, int i, long long ts, long long hs) {
+  const int tk = fast_div(i, f.by_group);
+  return (long long)(t.start + tk) * ts + (long long)(t.g * f.G + i - tk * f.G) * hs;
+}
+// The lane's row (a packed row, or none): queries as the second operand of the score product, bounds of its keys.
+template <int W>
+__device__ __forceinline__ void load_row(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int row, bool valid, int hh,
+                                         u32x4 (&qf)[W / 16], RowState<W>& st) {
   st.clear();
-  {
-    const int pos = q.start + tok + q.shift;
-    st.hi = valid ? min(pos, cap - 1) : -1;
-    st.lo = a.window > 0 ? pos - a.window + 1 : 0;
+  const int pos = t.start + fast_div(valid ? row : 0, f.by_group) + t.shift;
+  st.hi = valid ? min(pos, t.cap - 1) : -1;
+  st.lo = a.window > 0 ? pos - a.window + 1 : 0;
+  const uint16_t* qp = (const uint16_t*)a.q + (valid ? row_offset(f, t, row, a.q_ts, a.q_hs) : 0);
+#pragma unroll
+  for (int ks = 0; ks < W / 16; ++ks) {
+    const int d = ks * 16 + hh * 8;
+    qf[ks] = u32x4{0u, 0u, 0u, 0u};
+    if (valid && d < a.width) qf[ks] = *reinterpret_cast<const u32x4*>(qp + d);
   }
-  auto hide_missing = [&](int ks0, bool gone_pages) {
-    return [=](f32x16& s) {
-      if (!gone_pages) return;
-#pragma unroll 1
-      for (int i = 0; i < 32; ++i) {     // one page number at a time, the same for all lanes
-        const int key = ks0 + i;
-        bool gone = true;
-        if (key < khi) gone = (unsigned)table[fast_div(key, a.by_page)] >= (unsigned)a.pages;
-        if (gone) {
+  if (f.negate) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (acc_row(e, hh) == i) s[e] = -INFINITY;
-        }
-      }
-    };
-  };
+    for (int ks = 0; ks < W / 16; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[ks][e] ^= 0x80008000u;
+  }
+}
+// Keys of a subtile whose page does not exist.
+__device__ __forceinline__ void hide_missing(const PagedAttnArgs& a, const Tile& t, int ks0, int hh, f32x16& s) {
+  unsigned gone = 0u;
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i) {
+    const int key = ks0 + i;
+    if (key >= t.khi || (unsigned)t.table[fast_div(key, a.by_page)] >= (unsigned)a.pages) gone |= 1u << i;
+  }
+  gone >>= 4 * hh;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = gone & (1u << acc_row(e, 0)) ? -INFINITY : s[e];
+}
 
-  if (!q.chunk) {
-    // ---- few rows: subtile t of the piece belongs to wave t % 4 ----
-    constexpr int NP = SUB / 1024;
-    char* const kt = smem + wave * REGION;
-    char* const vt = kt + SUB;
-    const unsigned k_lds = lds0 + wave * REGION, v_lds = k_lds + SUB;
-    PageRows<W, NP, UNI> pr;
-    pr.init(a, table, g, klo, khi, lane);
-    int ks0 = k0 + wave * 32;
-    if (ks0 < k1) {
-      pr.fetch(ks0);
-      pr.template issue<false>(ks0, k_lds);
-      pr.template issue<true>(ks0, v_lds);
-    }
-    for (; ks0 < k1; ks0 += 128) {
-      const int next = ks0 + 128;
-      const bool more = next < k1;
-      const bool gone = pr.gone;
-      const bool mask = gone || ks0 + 31 > p_first || ks0 + 32 > cap || (a.window > 0 && ks0 < p_last - a.window + 1);
-      if (more) pr.fetch(next);
-      wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
-      subtile<T, W>(
-          kt, vt, ks0, mask, f.c, qf, st, lane,
-          [&]() {
-            wait_lds();         // the key fragments are in registers: their place takes the next subtile's
-            if (more) pr.template issue<false>(next, k_lds);
-          },
-          [&]() {
-            if (more) wait_dma_but<NP>();
-            else wait_dma_but<0>();
-          },
-          [&]() {
-            wait_lds();
-            if (more) pr.template issue<true>(next, v_lds);
-          },
-          hide_missing(ks0, gone));
-    }
-    // ---- merge the waves ----
-    const float l = sum_halves(st.l);
-    if (hh == 0) {
-      ml_s[wave][r32][0] = st.mb;
-      ml_s[wave][r32][1] = l;
-    }
-    __syncthreads();
-    float M = -INFINITY;
+// Few rows (at most 32) over keys [k0, k1), k0 a multiple of 32: subtile t belongs to wave t % 4, each wave has its own
+// part of LDS and its own running state; merged at the end, to the output (slot < 0) or to a slot of the workspace.
+// Leaves without a barrier behind its last reads of LDS.
+template <typename T, int W, bool UNI>
+__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, int slot,
+                                         char* smem, unsigned lds0, float (&ml_s)[4][32][2]) {
+  constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB, NP = SUB / 1024;
+  static_assert(REGION == 32 * W * 4, "a wave's two subtiles and its fp32 output share their place");
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));      // opaque: what follows from it is computed per run, not kept across the runs
+  const int lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* const kt = smem + wave * REGION;
+  char* const vt = kt + SUB;
+  const unsigned k_lds = lds0 + wave * REGION, v_lds = k_lds + SUB;
+  PageRows<W, NP, UNI> pr;
+  pr.init(a, t.table, t.g, t.klo, t.khi, lane);
+  int ks0 = k0 + wave * 32;
+  if (ks0 < k1) {
+    pr.fetch(ks0);
+    pr.template issue<false>(ks0, k_lds);
+    pr.template issue<true>(ks0, v_lds);
+  }
+  u32x4 qf[W / 16];
+  RowState<W> st;
+  const bool valid = r32 < t.nrows;
+  load_row<W>(a, f, t, t.rows0 + r32, valid, hh, qf, st);
+  for (; ks0 < k1; ks0 += kFewStep) {
+    const int next = ks0 + kFewStep;
+    const bool more = next < k1;
+    const bool gone = pr.gone;
+    const bool mask = gone || ks0 + 31 > t.p_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < t.p_last - a.window + 1);
+    if (more) pr.fetch(next);
+    wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
+    subtile<T, W>(
+        kt, vt, ks0, mask, f.c, qf, st, lane,
+        [&]() {
+          wait_lds();         // the key fragments are in registers: their place takes the next subtile's
+          if (more) pr.template issue<false>(next, k_lds);
+        },
+        [&]() {
+          if (more) wait_dma_but<NP>();
+          else wait_dma_but<0>();
+        },
+        [&]() {
+          wait_lds();
+          if (more) pr.template issue<true>(next, v_lds);
+        },
+        [&](f32x16& s) {
+          if (gone) hide_missing(a, t, ks0, hh, s);
+        });
+  }
+  // ---- merge the waves ----
+  const float l = sum_halves(st.l);
+  if (hh == 0) {
+    ml_s[wave][r32][0] = st.mb;
+    ml_s[wave][r32][1] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-      if (ml_s[w][r32][1] != 0.f) M = fmaxf(M, ml_s[w][r32][0]);
-    const float scale = l != 0.f ? __builtin_amdgcn_exp2f(st.mb - M) : 0.f;
-    char* const tile_o = smem + wave * REGION;
-    if (valid) {
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = l != 0.f ? st.o[dt][4 * g4 + e] * scale : 0.f;
-          *reinterpret_cast<f32x4*>(o_piece<W>(tile_o, r32, 8 * dt + 2 * g4 + hh)) = v;
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < nrows * (W / 8); i += kThreads) {
-      const int rr = i / (W / 8), d8 = i % (W / 8);
-      float M2 = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (ml_s[w][rr][1] != 0.f) M2 = fmaxf(M2, ml_s[w][rr][0]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (ml_s[w][rr][1] != 0.f) L += ml_s[w][rr][1] * __builtin_amdgcn_exp2f(ml_s[w][rr][0] - M2);
-      float o[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(o_piece<W>(smem + w * REGION, rr, 2 * d8));
-        const f32x4 y = *reinterpret_cast<const f32x4*>(o_piece<W>(smem + w * REGION, rr, 2 * d8 + 1));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[e] += x[e];
-          o[4 + e] += y[e];
-        }
-      }
-      if (np > 1) {
-        float* dst = f.part + ((long long)slot * f.slot_rows + rr) * W + 8 * d8;
-        store8(dst, o);
-        if (d8 == 0) {
-          f.ml[((long long)slot * f.slot_rows + rr) * 2] = M2;
-          f.ml[((long long)slot * f.slot_rows + rr) * 2 + 1] = L;
-        }
-      } else if (8 * d8 < a.width) {
-        const float inv = L != 0.f ? 1.f / L : 0.f;
-        u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = L != 0.f ? Frag<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
-        const int tk = fast_div(rows0 + rr, f.by_group), hd = g * f.G + rows0 + rr - tk * f.G;
-        *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(q.start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
-      }
-    }
-  } else {
-    // ---- chunks: the waves share 64-key tiles ----
-    constexpr int NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;    // pieces per wave; K and V tile
-    PageRows<W, NP, UNI> pr;
-    pr.init(a, table, g, klo, khi, lane);
-    constexpr int WROWS = 16;       // rows of a tile that a wave transfers
-    const int w_off = wave * WROWS;
-    const unsigned w_lds = lds0 + wave * NP * 1024;
-    const int wt_first = fast_div(min(rows0 + wave * 32, q.rows - 1), f.by_group);
-    const int wt_last = fast_div(min(rows0 + wave * 32 + 31, q.rows - 1), f.by_group);
-    const int wp_first = q.start + wt_first + q.shift, wp_last = q.start + wt_last + q.shift;
-    const bool wave_live = rows0 + wave * 32 < q.rows;
-    if (k0 < k1) {
-      pr.fetch(k0 + w_off);
-      pr.template issue<false>(k0 + w_off, w_lds);
-      pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
-    }
-    int stage = 0;
-    if (k0 + 64 < k1) pr.fetch(k0 + 64 + w_off);
-    for (int kt0 = k0; kt0 < k1; kt0 += 64) {
-      wait_dma_but<0>();
-      __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
-      const int next = kt0 + 64;
-      if (next < k1) {
-        const unsigned nb = w_lds + (stage ^ 1) * STAGE;
-        pr.template issue<false>(next + w_off, nb);
-        pr.template issue<true>(next + w_off, nb + 2 * SUB);
-        if (next + 64 < k1) pr.fetch(next + 64 + w_off);
-      }
-      const char* const kt = smem + stage * STAGE;
-      const char* const vt = kt + 2 * SUB;
-      stage ^= 1;
-      if (!wave_live) continue;
-#pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
-        const int ks0 = kt0 + 32 * sub;
-        if (ks0 > wp_last || ks0 >= khi) break;
-        if (a.window > 0 && ks0 + 31 < wp_first - a.window + 1) continue;
-        const bool mask = missing || ks0 + 31 > wp_first || ks0 + 32 > cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
-        subtile<T, W>(kt + sub * SUB, vt + sub * SUB, ks0, mask, f.c, qf, st, lane, [] {}, [] {}, [] {}, hide_missing(ks0, missing));
-      }
-    }
-    const float l = sum_halves(st.l);
-    __syncthreads();          // every wave is done with the tiles
-    char* const tile_o = smem + wave * REGION;
-    const float inv = np > 1 ? 1.f : (l != 0.f ? 1.f / l : 0.f);
+  for (int w = 0; w < 4; ++w)
+    if (ml_s[w][r32][1] != 0.f) M = fmaxf(M, ml_s[w][r32][0]);
+  const float scale = l != 0.f ? __builtin_amdgcn_exp2f(st.mb - M) : 0.f;
+  if (valid) {
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = l != 0.f ? st.o[dt][4 * g4 + e] * inv : 0.f;
-        *reinterpret_cast<f32x4*>(o_piece<W>(tile_o, r32, 8 * dt + 2 * g4 + hh)) = v;
+        for (int e = 0; e < 4; ++e) v[e] = l != 0.f ? st.o[dt][4 * g4 + e] * scale : 0.f;
+        *reinterpret_cast<f32x4*>(o_piece<W>(kt, r32, 8 * dt + 2 * g4 + hh)) = v;
       }
-    wait_lds();
-    const int mine = min(32, nrows - wave * 32);
-    for (int i = lane; i < mine * (W / 8); i += 64) {
-      const int rr = i / (W / 8), d8 = i % (W / 8);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(o_piece<W>(tile_o, rr, 2 * d8));
-      const f32x4 y = *reinterpret_cast<const f32x4*>(o_piece<W>(tile_o, rr, 2 * d8 + 1));
-      const int rw = wave * 32 + rr;
-      if (np > 1) {
-        float* dst = f.part + ((long long)slot * f.slot_rows + rw) * W + 8 * d8;
-        *reinterpret_cast<f32x4*>(dst) = x;
-        *reinterpret_cast<f32x4*>(dst + 4) = y;
-      } else if (8 * d8 < a.width) {
-        u32x4 w = {Frag<T>::pack(x[0], x[1]), Frag<T>::pack(x[2], x[3]), Frag<T>::pack(y[0], y[1]), Frag<T>::pack(y[2], y[3])};
-        const int tk = fast_div(rows0 + rw, f.by_group), hd = g * f.G + rows0 + rw - tk * f.G;
-        *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(q.start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
+  }
+  __syncthreads();
+  for (int i = tid; i < t.nrows * (W / 8); i += kThreads) {
+    const int rr = i / (W / 8), d8 = i % (W / 8);
+    float M2 = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (ml_s[w][rr][1] != 0.f) M2 = fmaxf(M2, ml_s[w][rr][0]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (ml_s[w][rr][1] != 0.f) L += ml_s[w][rr][1] * __builtin_amdgcn_exp2f(ml_s[w][rr][0] - M2);
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(o_piece<W>(smem + w * REGION, rr, 2 * d8));
+      const f32x4 y = *reinterpret_cast<const f32x4*>(o_piece<W>(smem + w * REGION, rr, 2 * d8 + 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e] += x[e];
+        o[4 + e] += y[e];
       }
     }
-    if (np > 1 && hh == 0 && r32 < mine) {
-      f.ml[((long long)slot * f.slot_rows + wave * 32 + r32) * 2] = st.mb;
-      f.ml[((long long)slot * f.slot_rows + wave * 32 + r32) * 2 + 1] = l;
+    if (slot >= 0) {
+      const long long at = (long long)slot * f.slot_rows + rr;
+      store8(f.part + at * W + 8 * d8, o);
+      if (d8 == 0) {
+        f.ml[at * 2] = M2;
+        f.ml[at * 2 + 1] = L;
+      }
+    } else if (8 * d8 < a.width) {
+      const float inv = L != 0.f ? 1.f / L : 0.f;
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = L != 0.f ? Frag<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
+      *reinterpret_cast<u32x4*>((uint16_t*)a.o + row_offset(f, t, t.rows0 + rr, a.o_ts, a.o_hs) + 8 * d8) = w;
     }
   }
-  if (np > 1 && tid == 0) {
-    int* m = f.meta + (long long)slot * 8;
-    m[0] = piece == 0 ? np : 0;      // the first piece of a tile leads the others, nkv slots apart
-    m[1] = q.start;
-    m[2] = rows0;
-    m[3] = nrows;
-    m[4] = g;
+}
+
+__device__ __forceinline__ void zero_rows_outside(const PagedAttnArgs& a) {
+  const int lo = a.R > 0 ? min(max(a.cu_q[0], 0), a.N) : a.N, hi = a.R > 0 ? min(max(a.cu_q[a.R], 0), a.N) : a.N;
+  const int rest = lo + a.N - max(hi, lo);
+  const long long total = (long long)rest * a.nh * a.width;
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
+    const int d = (int)(i % a.width), h = (int)((i / a.width) % a.nh);
+    int row = (int)(i / a.width / a.nh);
+    if (row >= lo) row += max(hi, lo) - lo;
+    ((uint16_t*)a.o)[(long long)row * a.o_ts + (long long)h * a.o_hs + d] = 0;
+  }
+}
+
+// What the second kernel needs to know of a slot: the pieces of its tile if it holds the first of them (0: it does not),
+// the tile, and where the others are: slot, then next + p * stride for p = 1 .. np - 1.
+__device__ __forceinline__ void write_meta(const FastArgs& f, int slot, int np, int start, int rows0, int nrows, int g, int next,
+                                           int stride) {
+  int* m = f.meta + (long long)slot * 8;
+  m[0] = np;
+  m[1] = start;
+  m[2] = rows0;
+  m[3] = nrows;
+  m[4] = g;
+  m[5] = next;
+  m[6] = stride;
+}
+
+template <typename T, int W, bool UNI>
+__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kernel(PagedAttnArgs a, FastArgs f) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float ml_s[4][32][2];
+  const int tid = threadIdx.x;
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
+  if (a.zero_rest) zero_rows_outside(a);
+  __shared__ Runs runs;
+  const int total = list_runs(a, f, runs);
+  const int id = blockIdx.x;
+  const int eff = min((int)gridDim.x, max((total + kMinSteps - 1) / kMinSteps, 1));
+  const int per = max((total + eff - 1) / eff, 1);
+  if (id == 0 && tid == 0) f.header[0] = 2 * eff;
+  if (id >= eff) return;
+  if (tid == 0) f.meta[(long long)(2 * id) * 8] = f.meta[(long long)(2 * id + 1) * 8] = 0;
+  int at = id * per;
+  const int end = min(at + per, total);
+  for (bool first_run = true; at < end; first_run = false) {
+    int first;
+    Request q;
+    const int r = find_run(a, f, runs, at, first, q);
+    if (r < 0) break;
+    const int steps = run_steps(q);
+    if (steps == 0) break;
+    const int run = (at - first) / steps, s0 = at - first - run * steps, s1 = min(steps, s0 + end - at);
+    const int g = run % a.nkv, rows0 = run / a.nkv * kFewRows;
+    if (s0 < 0 || run < 0 || rows0 >= q.rows) break;   // lengths that contradict each other
+    const Tile t = make_tile(a, f, q, r, g, rows0, kFewRows);
+    const int base = run_base(q), k0 = base + s0 * kFewStep, k1 = min(t.khi, base + s1 * kFewStep);
+    const bool whole = s0 == 0 && s1 == steps;
+    const int slot = whole ? -1 : 2 * id + (first_run ? 0 : 1);
+    if (!first_run) __syncthreads();                  // the last run's outputs have been read from LDS
+    few_rows<T, W, UNI>(a, f, t, k0, k1, slot, smem, lds0, ml_s);
+    if (!whole && s0 == 0 && tid == 0) {
+      const int last = (at + steps - 1) / per;        // the workgroup that has its end
+      write_meta(f, slot, last - id + 1, t.start, rows0, t.nrows, g, 2 * id, 2);
+    }
+    at += s1 - s0;
+  }
+}
+
+// Chunks, with few-row requests among them.
+template <typename T, int W, bool UNI>
+__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
+  constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float ml_s[4][32][2];
+  const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
+  if (a.zero_rest) zero_rows_outside(a);
+
+  // ---- this workgroup's item ----
+  const Item it = find_item(a, f, blockIdx.x, lane);
+  const int r = __builtin_amdgcn_readfirstlane(it.r);
+  if (r < 0) return;
+  const Request q = request(a, f, r);
+  const int np = __builtin_amdgcn_readfirstlane(it.np);
+  int slot = __builtin_amdgcn_readfirstlane(it.slot);
+  int j = __builtin_amdgcn_readfirstlane(it.j);
+  const int g = j % a.nkv;
+  j /= a.nkv;
+  const int piece = j % np;
+  const int tile = q.tiles - 1 - j / np;                 // the rows that see most come first
+  if (tile < 0 || j < 0 || (np > 1 && (unsigned)slot >= (unsigned)f.max_slots)) return;   // lengths that contradict each other
+  const int rows0 = tile * kChunkRows;
+  const Tile t = make_tile(a, f, q, r, g, rows0, q.chunk ? kChunkRows : kFewRows);
+  const int nrows = t.nrows, step = q.chunk ? kChunkStep : kFewStep;
+  const int k_base = t.klo & ~63;
+  const int span = ((t.khi - k_base + np - 1) / np + step - 1) / step * step;
+  const int k0 = k_base + piece * span, k1 = min(t.khi, k0 + span);
+  if (np > 1 && tid == 0) write_meta(f, slot, piece == 0 ? np : 0, q.start, rows0, nrows, g, slot, a.nkv);
+  if (!q.chunk) {
+    few_rows<T, W, UNI>(a, f, t, k0, k1, np > 1 ? slot : -1, smem, lds0, ml_s);
+    return;
+  }
+
+  // ---- a chunk: do all pages of the piece exist? ----
+  bool missing = false;
+  if (k1 > k0) {
+    const int c_lo = fast_div(max(k0, t.klo), a.by_page), c_hi = fast_div(k1 - 1, a.by_page);
+    for (int col = c_lo + tid; col <= c_hi; col += kThreads) missing |= (unsigned)t.table[col] >= (unsigned)a.pages;
+  }
+  missing = __syncthreads_or(missing);
+
+  // ---- the waves share 64-key tiles ----
+  constexpr int NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;    // transfers per wave and K or V tile; a K and a V tile
+  PageRows<W, NP, UNI> pr;
+  pr.init(a, t.table, g, t.klo, t.khi, lane);
+  const int w_off = wave * 16;                               // the 16 rows of a tile that the wave transfers
+  const unsigned w_lds = lds0 + wave * NP * 1024;
+  if (k0 < k1) {
+    pr.fetch(k0 + w_off);
+    pr.template issue<false>(k0 + w_off, w_lds);
+    pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
+  }
+  u32x4 qf[W / 16];
+  RowState<W> st;
+  load_row<W>(a, f, t, rows0 + wave * 32 + r32, rows0 + wave * 32 + r32 < q.rows, hh, qf, st);
+  const int wt_first = fast_div(min(rows0 + wave * 32, q.rows - 1), f.by_group);
+  const int wt_last = fast_div(min(rows0 + wave * 32 + 31, q.rows - 1), f.by_group);
+  const int wp_first = q.start + wt_first + q.shift, wp_last = q.start + wt_last + q.shift;
+  const bool wave_live = rows0 + wave * 32 < q.rows;
+  int stage = 0;
+  if (k0 + 64 < k1) pr.fetch(k0 + 64 + w_off);
+  for (int kt0 = k0; kt0 < k1; kt0 += 64) {
+    wait_dma_but<0>();
+    __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
+    const int next = kt0 + 64;
+    if (next < k1) {
+      const unsigned nb = w_lds + (stage ^ 1) * STAGE;
+      pr.template issue<false>(next + w_off, nb);
+      pr.template issue<true>(next + w_off, nb + 2 * SUB);
+      if (next + 64 < k1) pr.fetch(next + 64 + w_off);
+    }
+    const char* const kt = smem + stage * STAGE;
+    const char* const vt = kt + 2 * SUB;
+    stage ^= 1;
+    if (!wave_live) continue;
+#pragma unroll 1
+    for (int sub = 0; sub < 2; ++sub) {
+      const int ks0 = kt0 + 32 * sub;
+      if (ks0 > wp_last || ks0 >= t.khi) break;
+      if (a.window > 0 && ks0 + 31 < wp_first - a.window + 1) continue;
+      const bool mask = missing || ks0 + 31 > wp_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
+      subtile<T, W>(
+          kt + sub * SUB, vt + sub * SUB, ks0, mask, f.c, qf, st, lane, [] {}, [] {}, [] {},
+          [&](f32x16& s) {
+            if (missing) hide_missing(a, t, ks0, hh, s);
+          });
+    }
+  }
+  const float l = sum_halves(st.l);
+  __syncthreads();          // every wave is done with the tiles
+  char* const tile_o = smem + wave * REGION;
+  const float inv = np > 1 ? 1.f : (l != 0.f ? 1.f / l : 0.f);
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = l != 0.f ? st.o[dt][4 * g4 + e] * inv : 0.f;
+      *reinterpret_cast<f32x4*>(o_piece<W>(tile_o, r32, 8 * dt + 2 * g4 + hh)) = v;
+    }
+  wait_lds();
+  const int mine = min(32, nrows - wave * 32);
+  for (int i = lane; i < mine * (W / 8); i += 64) {
+    const int rr = i / (W / 8), d8 = i % (W / 8), rw = wave * 32 + rr;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(o_piece<W>(tile_o, rr, 2 * d8));
+    const f32x4 y = *reinterpret_cast<const f32x4*>(o_piece<W>(tile_o, rr, 2 * d8 + 1));
+    if (np > 1) {
+      float* dst = f.part + ((long long)slot * f.slot_rows + rw) * W + 8 * d8;
+      *reinterpret_cast<f32x4*>(dst) = x;
+      *reinterpret_cast<f32x4*>(dst + 4) = y;
+    } else if (8 * d8 < a.width) {
+      const u32x4 w = {Frag<T>::pack(x[0], x[1]), Frag<T>::pack(x[2], x[3]), Frag<T>::pack(y[0], y[1]), Frag<T>::pack(y[2], y[3])};
+      *reinterpret_cast<u32x4*>((uint16_t*)a.o + row_offset(f, t, rows0 + rw, a.o_ts, a.o_hs) + 8 * d8) = w;
+    }
+  }
+  if (np > 1 && hh == 0 && r32 < mine) {
+    const long long at = (long long)slot * f.slot_rows + wave * 32 + r32;
+    f.ml[at * 2] = st.mb;
+    f.ml[at * 2 + 1] = l;
   }
 }
 
@@ -943,6 +1095,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs
   if (slot >= f.header[0]) return;
   const int* meta = f.meta + (long long)slot * 8;
   const int np = meta[0], start = meta[1], rows0 = meta[2], nrows = min(meta[3] - (int)blockIdx.y * kJoinRows, kJoinRows), g = meta[4];
+  const int other = meta[5], stride = meta[6];
   if (np < 2 || nrows <= 0) return;
   const int row_b = blockIdx.y * kJoinRows, units = nrows * CPR;
   int groups = 1;
@@ -958,7 +1111,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int p = min(p0 + u * groups, np - 1);
-        const long long at = (long long)(slot + p * a.nkv) * f.slot_rows + rr;
+        const long long at = (long long)(p == 0 ? slot : other + p * stride) * f.slot_rows + rr;
         m[u] = f.ml[at * 2];
         l[u] = p0 + u * groups < np ? f.ml[at * 2 + 1] : 0.f;
         load8(f.part + at * W + 8 * d8, x[u]);
@@ -1027,13 +1180,19 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   Plan p;
   const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
   p.chunks = (long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows;
-  p.target = num_cus * 4;
-  if (const char* e = getenv("PA_TARGET")) p.target = atoi(e);
-  // tiles: one per request with rows, and one more for every 128 rows of a chunk
-  const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
-  p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
-  p.slots = (int)std::min<long long>(2ll * p.target, p.grid);
-  p.slot_rows = p.chunks ? kChunkRows : kFewRows;
+  if (p.chunks) {
+    p.target = num_cus * 4;
+    // tiles: one per request with rows, and one more for every 128 rows of a chunk
+    const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
+    p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
+    p.slots = (int)std::min<long long>(2ll * p.target, p.grid);
+    p.slot_rows = kChunkRows;
+  } else {
+    p.target = 0;
+    p.grid = num_cus * (W == 64 ? 3 : 2);      // the workgroups that fit the card at once
+    p.slots = 2 * p.grid;
+    p.slot_rows = kFewRows;
+  }
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.part = up((size_t)p.slots * p.slot_rows * W * 4);
   p.ml = up((size_t)p.slots * p.slot_rows * 8);
@@ -1045,14 +1204,14 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
 template <typename T, int W, bool UNI, bool CHUNKS>
 void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
   constexpr int lds = 4 * 2 * 32 * W * 2;
+  auto kernel = CHUNKS ? paged_attn_kernel<T, W, UNI> : paged_attn_few_kernel<T, W, UNI>;
   static bool set = false;       // above the default limit of dynamic LDS; the same value every time
   if (!set) {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, W, UNI, CHUNKS>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     set = true;
   }
-  if (a.R > kWaveRequests) hipLaunchKernelGGL(paged_attn_items_kernel, dim3(1), dim3(1024), 0, st, a, f);
-  hipLaunchKernelGGL((paged_attn_kernel<T, W, UNI, CHUNKS>), dim3(grid), dim3(kThreads), lds, st, a, f);
+  if (a.R > kWaveRequests) hipLaunchKernelGGL((paged_attn_items_kernel<CHUNKS>), dim3(1), dim3(1024), 0, st, a, f);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, st, a, f);
   hipLaunchKernelGGL((paged_attn_join_kernel<T, W>), dim3(f.max_slots, (f.slot_rows * (W / 8) + kThreads - 1) / kThreads),
                      dim3(kThreads), 0, st, a, f);
 }
