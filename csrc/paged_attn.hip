@@ -1,3 +1,6 @@
+#ifndef DPA_NS
+#define DPA_NS (W == 64 ? 2 : 1)
+#endif
 // Causal attention of the newest tokens of every request over its pages (gfx950). Row i of request r sits at position
 // pos = kv[r] - n[r] + i - cu[r] (n[r] = cu[r + 1] - cu[r]) and attends keys max(0, pos - window + 1) .. pos:
 //
@@ -651,9 +654,25 @@ __device__ __forceinline__ void place_non_finite(u32x4 (&vf)[2][W / 32], f32x16 
   }
 }
 
+// Whether any of the wave's values is not finite.
+template <typename T, int W>
+__device__ __forceinline__ bool not_finite(const u32x4 (&vf)[2][W / 32]) {
+  unsigned bad = 0u;
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+    for (int dt = 0; dt < W / 32; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bad |= (vf[s2][dt][j] & Frag<T>::kExp) + Frag<T>::kExpOne;   // carries into the sign
+  return __any((bad & 0x80008000u) != 0u);
+}
+
 // A 32-key subtile: keys [ks0, ks0 + 32) in the LDS tiles kt, vt. mask: some of them are hidden from some row of the wave.
-template <typename T, int W, class AfterK, class BeforeV, class AfterV, class Hidden>
-__device__ __forceinline__ void subtile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
+// RARE: with place_non_finite() and the caller's `hidden` (keys of missing pages). Without it the return value says
+// that the former was called for; the two are kept apart because the rare code's registers would be spilled in the
+// common loop, and a spill's reload waits for the transfers in flight (737 -> 1232 us on the 16k prefill).
+template <typename T, int W, bool RARE, class AfterK, class BeforeV, class AfterV, class Hidden>
+__device__ __forceinline__ bool subtile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
                                         RowState<W>& st, int lane, AfterK after_k, BeforeV before_v, AfterV after_v,
                                         Hidden hidden) {
   typedef Frag<T> F;
@@ -675,7 +694,7 @@ __device__ __forceinline__ void subtile(const char* kt, const char* vt, int ks0,
       const int key = acc_row(i, hh);
       if (key < lo_rel || key > hi_rel) s[i] = -INFINITY;
     }
-    hidden(s);
+    if (RARE) hidden(s);
   }
   float mx = s[0];
 #pragma unroll
@@ -707,15 +726,10 @@ __device__ __forceinline__ void subtile(const char* kt, const char* vt, int ks0,
   }
   st.l += rs;
   after_v();
+  bool rare = false;
   if (mask) {
-    unsigned bad = 0u;
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bad |= (vf[s2][dt][j] & F::kExp) + F::kExpOne;
-    if (__any((bad & 0x80008000u) != 0u)) place_non_finite<T, W>(vf, st.o, lo_rel, hi_rel, hh);
+    rare = not_finite<T, W>(vf);
+    if (RARE && rare) place_non_finite<T, W>(vf, st.o, lo_rel, hi_rel, hh);
   }
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
@@ -725,6 +739,104 @@ __device__ __forceinline__ void subtile(const char* kt, const char* vt, int ks0,
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) st.o[dt] = F::mfma(vf[s2][dt], pb, st.o[dt]);
   }
+  return rare;
+}
+
+// NS 32-key subtiles of a chunk's tile, from key ks0 on. No maximum is taken as a rule: the probabilities come from the
+// reference as it is, and what they sum to says whether it still serves (fp32 sums and the 16-bit operand keep their
+// relative precision whatever the magnitude; kSumMax keeps fp16 finite). If it does not, or a row has none yet, the
+// scores are computed again and the reference moves to their maximum.
+template <typename T, int W, int NS, bool RARE, class Hidden>
+__device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
+                                           RowState<W>& st, int lane, Hidden hidden) {
+  typedef Frag<T> F;
+  constexpr int NK = W / 16, ND = W / 32, SUB = 32 * W * 2;
+  constexpr float kSumMax = F::kBias ? 32768.f : 1.0e9f;
+  const int r = lane & 31, hh = lane >> 5;
+  f32x16 s[NS];
+  auto scores = [&]() {
+#pragma unroll
+    for (int h = 0; h < NS; ++h) {
+      u32x4 kf[NK];
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) kf[ks] = __builtin_bit_cast(u32x4, row_frag<W>(kt + h * SUB, r, ks, hh));
+      __builtin_amdgcn_sched_barrier(0);     // all fragments requested before the first product
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) s[h] = F::mfma(kf[ks], qf[ks], s[h]);
+    }
+    if (mask) {
+      const int lo_rel = st.lo - ks0 - 4 * hh, hi_rel = st.hi - ks0 - 4 * hh;
+#pragma unroll
+      for (int h = 0; h < NS; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = 32 * h + acc_row(i, 0);
+          if (key < lo_rel || key > hi_rel) s[h][i] = -INFINITY;
+        }
+      if (RARE)
+#pragma unroll
+        for (int h = 0; h < NS; ++h) hidden(ks0 + 32 * h, s[h]);
+    }
+  };
+  auto weights = [&]() {
+    const float base = st.mb == -INFINITY ? 0.f : st.mb;      // a row that sees nothing yet: every s is -inf
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < NS; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], c, -base));
+        sum[i & 1] += s[h][i];
+      }
+    return sum[0] + sum[1];
+  };
+  scores();
+  float rs = weights();
+  if (!__all(rs <= kSumMax && (st.mb != -INFINITY || st.hi < 0))) {
+    scores();
+    float mx = s[0][0];
+#pragma unroll
+    for (int h = 0; h < NS; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
+    const float to = max_halves(mx) * c - (float)F::kBias;
+    const bool move = to > st.mb;
+    const float alpha = move ? __builtin_amdgcn_exp2f(st.mb - to) : 1.f;
+    st.mb = move ? to : st.mb;
+    st.l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[dt][i] *= alpha;
+    rs = weights();
+  }
+  st.l += rs;
+  bool rare = false;
+#pragma unroll
+  for (int h = 0; h < NS; ++h) {
+    u32x4 vf[2][ND];
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) vf[s2][dt] = __builtin_bit_cast(u32x4, tr_frag<W>(vt + h * SUB, 0, s2, dt, lane));
+    __builtin_amdgcn_sched_barrier(0);
+    if (mask) {
+      const bool bad = not_finite<T, W>(vf);
+      rare |= bad;
+      if (RARE && bad) place_non_finite<T, W>(vf, st.o, st.lo - ks0 - 32 * h, st.hi - ks0 - 32 * h, hh);
+    }
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      u32x4 pb;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pb[j] = F::pack(s[h][8 * s2 + 2 * j], s[h][8 * s2 + 2 * j + 1]);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) st.o[dt] = F::mfma(vf[s2][dt], pb, st.o[dt]);
+    }
+  }
+  return rare;
 }
 
 // fp32 output tile [32 rows][W] of a wave in LDS; 16-byte pieces XORed with the row against bank conflicts.
@@ -796,33 +908,23 @@ __device__ __forceinline__ void hide_missing(const PagedAttnArgs& a, const Tile&
   for (int e = 0; e < 16; ++e) s[e] = gone & (1u << acc_row(e, 0)) ? -INFINITY : s[e];
 }
 
-// Few rows (at most 32) over keys [k0, k1), k0 a multiple of 32: subtile t belongs to wave t % 4, each wave has its own
-// part of LDS and its own running state; merged at the end, to the output (slot < 0) or to a slot of the workspace.
-// Leaves without a barrier behind its last reads of LDS.
-template <typename T, int W, bool UNI>
-__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, int slot,
-                                         char* smem, unsigned lds0, float (&ml_s)[4][32][2]) {
-  constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB, NP = SUB / 1024;
-  static_assert(REGION == 32 * W * 4, "a wave's two subtiles and its fp32 output share their place");
-  int tid = threadIdx.x;
-  asm volatile("" : "+v"(tid));      // opaque: what follows from it is computed per run, not kept across the runs
-  const int lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  char* const kt = smem + wave * REGION;
+// One wave's subtiles of few rows: every fourth from ks0 on. Returns whether they need the RARE form.
+template <typename T, int W, bool UNI, bool RARE>
+__device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int ks0, int k1, bool valid,
+                                         char* kt, unsigned k_lds, int lane, u32x4 (&qf)[W / 16], RowState<W>& st) {
+  constexpr int SUB = 32 * W * 2, NP = SUB / 1024;
+  const int hh = lane >> 5;
   char* const vt = kt + SUB;
-  const unsigned k_lds = lds0 + wave * REGION, v_lds = k_lds + SUB;
+  const unsigned v_lds = k_lds + SUB;
   PageRows<W, NP, UNI> pr;
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
-  int ks0 = k0 + wave * 32;
   if (ks0 < k1) {
     pr.fetch(ks0);
     pr.template issue<false>(ks0, k_lds, f.stream);
     pr.template issue<true>(ks0, v_lds, f.stream);
   }
-  u32x4 qf[W / 16];
-  RowState<W> st;
-  const bool valid = r32 < t.nrows;
-  load_row<W>(a, f, t, t.rows0 + r32, valid, hh, qf, st);
+  load_row<W>(a, f, t, t.rows0 + (lane & 31), valid, hh, qf, st);
+  bool rare = false;
   for (; ks0 < k1; ks0 += kFewStep) {
     const int next = ks0 + kFewStep;
     const bool more = next < k1;
@@ -830,7 +932,8 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs&
     const bool mask = gone || ks0 + 31 > t.p_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < t.p_last - a.window + 1);
     if (more) pr.fetch(next);
     wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
-    subtile<T, W>(
+    rare |= gone;
+    rare |= subtile<T, W, RARE>(
         kt, vt, ks0, mask, f.c, qf, st, lane,
         [&]() {
           wait_lds();         // the key fragments are in registers: their place takes the next subtile's
@@ -848,6 +951,28 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs&
           if (gone) hide_missing(a, t, ks0, hh, s);
         });
   }
+  return rare;
+}
+
+// Few rows (at most 32) over keys [k0, k1), k0 a multiple of 32: subtile t belongs to wave t % 4, each wave has its own
+// part of LDS and its own running state; merged at the end, to the output (slot < 0) or to a slot of the workspace.
+// Leaves without a barrier behind its last reads of LDS.
+template <typename T, int W, bool UNI>
+__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, int slot,
+                                         char* smem, unsigned lds0, float (&ml_s)[4][32][2]) {
+  constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB;
+  static_assert(REGION == 32 * W * 4, "a wave's two subtiles and its fp32 output share their place");
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));      // opaque: what follows from it is computed per run, not kept across the runs
+  const int lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* const kt = smem + wave * REGION;
+  const unsigned k_lds = lds0 + wave * REGION;
+  u32x4 qf[W / 16];
+  RowState<W> st;
+  const bool valid = r32 < t.nrows;
+  if (few_loop<T, W, UNI, false>(a, f, t, k0 + wave * 32, k1, valid, kt, k_lds, lane, qf, st))
+    few_loop<T, W, UNI, true>(a, f, t, k0 + wave * 32, k1, valid, kt, k_lds, lane, qf, st);
   // ---- merge the waves ----
   const float l = sum_halves(st.l);
   if (hh == 0) {
@@ -978,6 +1103,58 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kern
   }
 }
 
+// 128 rows over keys [k0, k1), k0 a multiple of 64: the waves share 64-key tiles. Returns whether the RARE form is needed.
+template <typename T, int W, bool UNI, bool RARE>
+__device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, bool missing,
+                                           char* smem, unsigned lds0, int wave, int lane, u32x4 (&qf)[W / 16], RowState<W>& st) {
+  constexpr int SUB = 32 * W * 2, NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;   // transfers per wave and tile; a K and a V tile
+  constexpr int NS = DPA_NS;
+  const int r32 = lane & 31, hh = lane >> 5;
+  PageRows<W, NP, UNI> pr;
+  pr.init(a, t.table, t.g, t.klo, t.khi, lane);
+  const int w_off = wave * 16;                               // the 16 rows of a tile that the wave transfers
+  const unsigned w_lds = lds0 + wave * NP * 1024;
+  if (k0 < k1) {
+    pr.fetch(k0 + w_off);
+    pr.template issue<false>(k0 + w_off, w_lds);
+    pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
+  }
+  const int row = t.rows0 + wave * 32;
+  load_row<W>(a, f, t, row + r32, row + r32 < t.rows, hh, qf, st);
+  const int wp_first = t.start + fast_div(min(row, t.rows - 1), f.by_group) + t.shift;
+  const int wp_last = t.start + fast_div(min(row + 31, t.rows - 1), f.by_group) + t.shift;
+  const bool wave_live = row < t.rows;
+  bool rare = false;
+  int stage = 0;
+  if (k0 + 64 < k1) pr.fetch(k0 + 64 + w_off);
+  for (int kt0 = k0; kt0 < k1; kt0 += 64) {
+    wait_dma_but<0>();
+    __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
+    const int next = kt0 + 64;
+    if (next < k1) {
+      const unsigned nb = w_lds + (stage ^ 1) * STAGE;
+      pr.template issue<false>(next + w_off, nb);
+      pr.template issue<true>(next + w_off, nb + 2 * SUB);
+      if (next + 64 < k1) pr.fetch(next + 64 + w_off);
+    }
+    const char* const kt = smem + stage * STAGE;
+    const char* const vt = kt + 2 * SUB;
+    stage ^= 1;
+    if (!wave_live) continue;
+#pragma unroll 1
+    for (int ks0 = kt0; ks0 < kt0 + 64; ks0 += 32 * NS) {
+      if (ks0 > wp_last || ks0 >= t.khi) break;
+      if (a.window > 0 && ks0 + 32 * NS - 1 < wp_first - a.window + 1) continue;
+      const bool mask = missing || ks0 + 32 * NS - 1 > wp_first || ks0 + 32 * NS > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
+      const int at = (ks0 - kt0) * W * 2;
+      rare |= chunk_tile<T, W, NS, RARE>(kt + at, vt + at, ks0, mask, f.c, qf, st, lane, [&](int k, f32x16& s) {
+        if (missing) hide_missing(a, t, k, hh, s);
+      });
+    }
+  }
+  return rare;
+}
+
 // Chunks, with few-row requests among them.
 template <typename T, int W, bool UNI>
 __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
@@ -1022,53 +1199,11 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(P
   }
   missing = __syncthreads_or(missing);
 
-  // ---- the waves share 64-key tiles ----
-  constexpr int NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;    // transfers per wave and K or V tile; a K and a V tile
-  PageRows<W, NP, UNI> pr;
-  pr.init(a, t.table, g, t.klo, t.khi, lane);
-  const int w_off = wave * 16;                               // the 16 rows of a tile that the wave transfers
-  const unsigned w_lds = lds0 + wave * NP * 1024;
-  if (k0 < k1) {
-    pr.fetch(k0 + w_off);
-    pr.template issue<false>(k0 + w_off, w_lds);
-    pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
-  }
   u32x4 qf[W / 16];
   RowState<W> st;
-  load_row<W>(a, f, t, rows0 + wave * 32 + r32, rows0 + wave * 32 + r32 < q.rows, hh, qf, st);
-  const int wt_first = fast_div(min(rows0 + wave * 32, q.rows - 1), f.by_group);
-  const int wt_last = fast_div(min(rows0 + wave * 32 + 31, q.rows - 1), f.by_group);
-  const int wp_first = q.start + wt_first + q.shift, wp_last = q.start + wt_last + q.shift;
-  const bool wave_live = rows0 + wave * 32 < q.rows;
-  int stage = 0;
-  if (k0 + 64 < k1) pr.fetch(k0 + 64 + w_off);
-  for (int kt0 = k0; kt0 < k1; kt0 += 64) {
-    wait_dma_but<0>();
-    __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
-    const int next = kt0 + 64;
-    if (next < k1) {
-      const unsigned nb = w_lds + (stage ^ 1) * STAGE;
-      pr.template issue<false>(next + w_off, nb);
-      pr.template issue<true>(next + w_off, nb + 2 * SUB);
-      if (next + 64 < k1) pr.fetch(next + 64 + w_off);
-    }
-    const char* const kt = smem + stage * STAGE;
-    const char* const vt = kt + 2 * SUB;
-    stage ^= 1;
-    if (!wave_live) continue;
-#pragma unroll 1
-    for (int sub = 0; sub < 2; ++sub) {
-      const int ks0 = kt0 + 32 * sub;
-      if (ks0 > wp_last || ks0 >= t.khi) break;
-      if (a.window > 0 && ks0 + 31 < wp_first - a.window + 1) continue;
-      const bool mask = missing || ks0 + 31 > wp_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
-      subtile<T, W>(
-          kt + sub * SUB, vt + sub * SUB, ks0, mask, f.c, qf, st, lane, [] {}, [] {}, [] {},
-          [&](f32x16& s) {
-            if (missing) hide_missing(a, t, ks0, hh, s);
-          });
-    }
-  }
+  bool rare = missing;
+  if (!rare) rare = __syncthreads_or(chunk_loop<T, W, UNI, false>(a, f, t, k0, k1, false, smem, lds0, wave, lane, qf, st));
+  if (rare) chunk_loop<T, W, UNI, true>(a, f, t, k0, k1, missing, smem, lds0, wave, lane, qf, st);
   const float l = sum_halves(st.l);
   __syncthreads();          // every wave is done with the tiles
   char* const tile_o = smem + wave * REGION;
