@@ -1,5 +1,11 @@
 #ifndef DPA_NS
-#define DPA_NS (W == 64 ? 2 : 1)
+#define DPA_NS (W == 64 ? 1 : 2)
+#endif
+#ifndef DPA_T
+#define DPA_T 2
+#endif
+#ifndef DPA_LB
+#define DPA_LB (W==64?3:2)
 #endif
 // Causal attention of the newest tokens of every request over its pages (gfx950). Row i of request r sits at position
 // pos = kv[r] - n[r] + i - cu[r] (n[r] = cu[r + 1] - cu[r]) and attends keys max(0, pos - window + 1) .. pos:
@@ -134,8 +140,7 @@ constexpr int kFewStep = 128, kChunkStep = 64;      // keys a workgroup advances
 template <typename T> struct Frag;
 template <> struct Frag<bf16_t> {
   static constexpr int kBias = 0;
-  static constexpr unsigned kExp = 0x7f807f80u, kExpOne = 0x00800080u, kInf = 0x7f80u, kSign = 0x8000u;
-  static constexpr unsigned kOne = 0x3f80u, k64 = 0x4280u, k4096 = 0x4580u;
+  static constexpr unsigned kExp = 0x7f807f80u, kExpOne = 0x00800080u;     // both halves' exponents, and their last bits
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfrag, a), __builtin_bit_cast(bfrag, b), c, 0, 0, 0);
   }
@@ -143,8 +148,7 @@ template <> struct Frag<bf16_t> {
 };
 template <> struct Frag<half_t> {
   static constexpr int kBias = 6;
-  static constexpr unsigned kExp = 0x7c007c00u, kExpOne = 0x04000400u, kInf = 0x7c00u, kSign = 0x8000u;
-  static constexpr unsigned kOne = 0x3c00u, k64 = 0x5400u, k4096 = 0x6c00u;
+  static constexpr unsigned kExp = 0x7c007c00u, kExpOne = 0x04000400u;
   typedef __attribute__((ext_vector_type(8))) _Float16 half8;
   typedef __attribute__((ext_vector_type(2))) _Float16 half2_t;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -484,19 +488,22 @@ __device__ __forceinline__ void dma_lane(unsigned long long addr, unsigned dst) 
       : "memory", "m0");
 }
 
-// Rows of pages -> LDS. A piece is RPP rows of W columns. When the page size is a multiple of RPP and the row fills the
-// tile (UNI), a piece lies in one page: the page number and the address come from scalar registers.
-template <int W, int NP, bool UNI>
+// NP pieces (1 KiB transfers of RPP rows of W columns) of pages -> LDS. RUN: rows that are known to lie in one page, since
+// the page size is a multiple of it and the row fills the tile: the page number and the address of a run come from
+// scalar registers, its pieces are lane offsets. RUN = 0: nothing is known, every lane looks its row up (any page size,
+// rows narrower than the tile).
+template <int W, int NP, int RUN>
 struct PageRows {
-  static constexpr int CPR = W / 8, RPP = 64 / CPR;
+  static constexpr int CPR = W / 8, RPP = 64 / CPR, PER = RUN > 0 ? RUN / RPP : 1, NR = NP / PER;    // pieces per run, runs
   static constexpr int VAR = W == 128 ? 4 : 2;      // the swizzle of a piece repeats after VAR pieces
+  static constexpr int OFF = PER > VAR ? PER : VAR;
   const PagedAttnArgs* a;
   const int* table;       // the request's row
   unsigned long long kb, vb;
   int klo, khi, lane;
   bool gone;              // a page of the rows fetched last does not exist
-  unsigned kv_off[2][VAR];
-  int pg[NP];
+  unsigned kv_off[2][OFF];
+  int pg[RUN > 0 ? NR : NP];
 
   __device__ __forceinline__ void init(const PagedAttnArgs& args, const int* t, int g, int lo, int hi, int lane_) {
     a = &args;
@@ -508,61 +515,67 @@ struct PageRows {
     kb = (unsigned long long)args.k + 2ull * (unsigned long long)(g * args.k_hs);
     vb = (unsigned long long)args.v + 2ull * (unsigned long long)(g * args.v_hs);
 #pragma unroll
-    for (int v = 0; v < VAR; ++v) {
+    for (int v = 0; v < OFF; ++v) {
       const int row = v * RPP + lane / CPR;
       const unsigned col = 16u * swz<W>(row, lane % CPR);
-      kv_off[0][v] = (unsigned)(lane / CPR) * (unsigned)(2 * args.k_rs) + col;
-      kv_off[1][v] = (unsigned)(lane / CPR) * (unsigned)(2 * args.v_rs) + col;
+      const int in_run = (v % PER) * RPP + lane / CPR;
+      kv_off[0][v] = (unsigned)in_run * (unsigned)(2 * args.k_rs) + col;
+      kv_off[1][v] = (unsigned)in_run * (unsigned)(2 * args.v_rs) + col;
     }
   }
-  __device__ __forceinline__ bool whole(int ks0) const { return UNI && ks0 >= klo && ks0 + NP * RPP <= khi; }
-  // page numbers of the rows [ks0, ks0 + NP * RPP), for the issue() of those rows
+  __device__ __forceinline__ bool whole(int ks0) const { return RUN > 0 && ks0 >= klo && ks0 + NP * RPP <= khi; }
+  // page numbers of the rows [ks0, ks0 + NP * RPP), for the issue() of those rows; known() waits for them
   __device__ __forceinline__ void fetch(int ks0) {
+    if (whole(ks0)) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int col = fast_div(ks0 + i * PER * RPP, a->by_page);
+        typedef const __attribute__((address_space(4))) int* scalar_ptr;
+        pg[i] = *(scalar_ptr)(unsigned long long)(table + __builtin_amdgcn_readfirstlane(col));
+      }
+    } else if (RUN == 0) {
+#pragma unroll
+      for (int pc = 0; pc < NP; ++pc) pg[pc] = lane_page(ks0 + pc * RPP + lane / CPR);
+    }
+  }
+  __device__ __forceinline__ void known(int ks0) {
     bool bad = false;
     if (whole(ks0)) {
 #pragma unroll
-      for (int pc = 0; pc < NP; ++pc) {
-        const int col = fast_div(ks0 + pc * RPP, a->by_page);
-        typedef const __attribute__((address_space(4))) int* scalar_ptr;
-        pg[pc] = *(scalar_ptr)(unsigned long long)(table + __builtin_amdgcn_readfirstlane(col));
-      }
-#pragma unroll
-      for (int pc = 0; pc < NP; ++pc) bad |= (unsigned)pg[pc] >= (unsigned)a->pages;
+      for (int i = 0; i < NR; ++i) bad |= (unsigned)pg[i] >= (unsigned)a->pages;
     } else {
 #pragma unroll
       for (int pc = 0; pc < NP; ++pc) {
-        const int key = ks0 + pc * RPP + lane / CPR;
-        pg[pc] = -1;
-        if (key >= klo && key < khi) {
-          pg[pc] = table[fast_div(key, a->by_page)];
-          bad |= (unsigned)pg[pc] >= (unsigned)a->pages;
-        }
+        const int key = ks0 + pc * RPP + lane / CPR, p = RUN == 0 ? pg[pc] : lane_page(key);
+        bad |= key >= klo && key < khi && (unsigned)p >= (unsigned)a->pages;
       }
       bad = __any(bad);
     }
     gone = bad;
   }
+  __device__ __forceinline__ int lane_page(int key) const {
+    return key >= klo && key < khi ? table[fast_div(key, a->by_page)] : -1;
+  }
   // `stream` (few rows over pools past the memory-side cache: every byte is read once): without a place in the caches
   template <bool V>
   __device__ __forceinline__ void issue(int ks0, unsigned lds, bool stream = false) const {
     const unsigned long long base = V ? vb : kb;
-    const unsigned long long ps = 2ull * (unsigned long long)(V ? a->v_ps : a->k_ps);
-    const unsigned rs = 2u * (unsigned)(V ? a->v_rs : a->k_rs);
+    const unsigned ps = 2u * (unsigned)(V ? a->v_ps : a->k_ps), rs = 2u * (unsigned)(V ? a->v_rs : a->k_rs);
     if (whole(ks0) && !gone) {
-      unsigned long long from[NP];
+      unsigned long long from[NR];
 #pragma unroll
-      for (int pc = 0; pc < NP; ++pc) {
-        const int key = ks0 + pc * RPP;
-        const int row = __builtin_amdgcn_readfirstlane(key - fast_div(key, a->by_page) * a->page);
-        const unsigned p = __builtin_amdgcn_readfirstlane(pg[pc]);
-        from[pc] = base + p * ps + (unsigned)row * rs;
+      for (int i = 0; i < NR; ++i) {
+        const int key = ks0 + i * PER * RPP;
+        const unsigned row = __builtin_amdgcn_readfirstlane(key - fast_div(key, a->by_page) * a->page);
+        const unsigned p = __builtin_amdgcn_readfirstlane(pg[i]);
+        from[i] = base + (unsigned long long)p * ps + row * rs;
       }
       if (stream) {
 #pragma unroll
-        for (int pc = 0; pc < NP; ++pc) dma_uniform<true>(from[pc], kv_off[V][pc % VAR], lds + pc * 1024);
+        for (int pc = 0; pc < NP; ++pc) dma_uniform<true>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);
       } else {
 #pragma unroll
-        for (int pc = 0; pc < NP; ++pc) dma_uniform<false>(from[pc], kv_off[V][pc % VAR], lds + pc * 1024);
+        for (int pc = 0; pc < NP; ++pc) dma_uniform<false>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);
       }
       return;
     }
@@ -571,9 +584,10 @@ struct PageRows {
       const int row = pc * RPP + lane / CPR, key = ks0 + row;
       const int ch = swz<W>(row, lane % CPR);
       unsigned long long addr = (unsigned long long)zero_row + 16u * ch;
+      const int p = RUN == 0 ? pg[pc] : lane_page(key);
       const int col = fast_div(max(key, 0), a->by_page);
-      if ((unsigned)pg[pc] < (unsigned)a->pages && key >= klo && key < khi && ch * 8 < a->width)
-        addr = base + (unsigned)pg[pc] * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
+      if ((unsigned)p < (unsigned)a->pages && key >= klo && key < khi && ch * 8 < a->width)
+        addr = base + (unsigned long long)(unsigned)p * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
       dma_lane(addr, lds + pc * 1024);
     }
   }
@@ -609,51 +623,6 @@ __device__ __forceinline__ float sum_halves(float x) {
   return u + v;
 }
 
-// Values that are not finite, in a subtile some of whose keys are hidden from some rows: 0 * inf would reach those rows.
-// They leave the fragments, and a product of the visibility (0 / 1) with codes (1: +inf, 64: -inf, 4096: NaN; at most 32
-// keys, so the counts do not run into each other) says which outputs they belong in.
-template <typename T, int W>
-__device__ __forceinline__ void place_non_finite(u32x4 (&vf)[2][W / 32], f32x16 (&o)[W / 32], int lo_rel, int hi_rel, int hh) {
-  typedef Frag<T> F;
-  u32x4 seen[2];
-  const unsigned span = (unsigned)(hi_rel - lo_rel);     // hi_rel < lo_rel: no key, and no difference below reaches it
-#pragma unroll
-  for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned k0 = (unsigned)(acc_row(8 * s2 + 2 * j, hh) - lo_rel);
-      seen[s2][j] = hi_rel < lo_rel ? 0u : (k0 <= span ? F::kOne : 0u) | (k0 + 1u <= span ? F::kOne << 16 : 0u);
-    }
-  // one 16-bit value: code, and whether it stays
-  auto code_of = [](unsigned x) {
-    return (x & F::kInf) != F::kInf ? 0u : (x & 0x7fffu) != F::kInf ? F::k4096 : (x & F::kSign) ? F::k64 : F::kOne;
-  };
-#pragma unroll
-  for (int dt = 0; dt < W / 32; ++dt) {
-    f32x16 code;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) code[i] = 0.f;
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      u32x4 cw;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned w = vf[s2][dt][j], lo = code_of(w & 0xffffu), hi = code_of(w >> 16);
-        vf[s2][dt][j] = (lo ? 0u : w & 0xffffu) | (hi ? 0u : w & 0xffff0000u);
-        cw[j] = lo | hi << 16;
-      }
-      code = F::mfma(cw, seen[s2], code);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int n = (int)code[i], pos = n & 63, neg = n & 4032;
-      const float one_sign = pos ? INFINITY : -INFINITY;
-      const float what = n >= 4096 || (pos && neg) ? __builtin_nanf("") : one_sign;
-      o[dt][i] += n != 0 ? what : 0.f;
-    }
-  }
-}
-
 // Whether any of the wave's values is not finite.
 template <typename T, int W>
 __device__ __forceinline__ bool not_finite(const u32x4 (&vf)[2][W / 32]) {
@@ -667,14 +636,11 @@ __device__ __forceinline__ bool not_finite(const u32x4 (&vf)[2][W / 32]) {
   return __any((bad & 0x80008000u) != 0u);
 }
 
-// A 32-key subtile: keys [ks0, ks0 + 32) in the LDS tiles kt, vt. mask: some of them are hidden from some row of the wave.
-// RARE: with place_non_finite() and the caller's `hidden` (keys of missing pages). Without it the return value says
-// that the former was called for; the two are kept apart because the rare code's registers would be spilled in the
-// common loop, and a spill's reload waits for the transfers in flight (737 -> 1232 us on the 16k prefill).
-template <typename T, int W, bool RARE, class AfterK, class BeforeV, class AfterV, class Hidden>
+// A 32-key subtile: keys [ks0, ks0 + 32) in the LDS tiles kt, vt. mask: some of them are hidden from some row of the wave;
+// returns whether one of their values is not finite then (exact_rows).
+template <typename T, int W, class AfterK, class BeforeV, class AfterV>
 __device__ __forceinline__ bool subtile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
-                                        RowState<W>& st, int lane, AfterK after_k, BeforeV before_v, AfterV after_v,
-                                        Hidden hidden) {
+                                        RowState<W>& st, int lane, AfterK after_k, BeforeV before_v, AfterV after_v) {
   typedef Frag<T> F;
   constexpr int NK = W / 16, ND = W / 32;
   const int r = lane & 31, hh = lane >> 5;
@@ -694,7 +660,6 @@ __device__ __forceinline__ bool subtile(const char* kt, const char* vt, int ks0,
       const int key = acc_row(i, hh);
       if (key < lo_rel || key > hi_rel) s[i] = -INFINITY;
     }
-    if (RARE) hidden(s);
   }
   float mx = s[0];
 #pragma unroll
@@ -727,10 +692,7 @@ __device__ __forceinline__ bool subtile(const char* kt, const char* vt, int ks0,
   st.l += rs;
   after_v();
   bool rare = false;
-  if (mask) {
-    rare = not_finite<T, W>(vf);
-    if (RARE && rare) place_non_finite<T, W>(vf, st.o, lo_rel, hi_rel, hh);
-  }
+  if (mask) rare = not_finite<T, W>(vf);
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
     u32x4 pb;
@@ -746,9 +708,9 @@ __device__ __forceinline__ bool subtile(const char* kt, const char* vt, int ks0,
 // reference as it is, and what they sum to says whether it still serves (fp32 sums and the 16-bit operand keep their
 // relative precision whatever the magnitude; kSumMax keeps fp16 finite). If it does not, or a row has none yet, the
 // scores are computed again and the reference moves to their maximum.
-template <typename T, int W, int NS, bool RARE, class Hidden>
+template <typename T, int W, int NS>
 __device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
-                                           RowState<W>& st, int lane, Hidden hidden) {
+                                           RowState<W>& st, int lane) {
   typedef Frag<T> F;
   constexpr int NK = W / 16, ND = W / 32, SUB = 32 * W * 2;
   constexpr float kSumMax = F::kBias ? 32768.f : 1.0e9f;
@@ -775,9 +737,6 @@ __device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int k
           const int key = 32 * h + acc_row(i, 0);
           if (key < lo_rel || key > hi_rel) s[h][i] = -INFINITY;
         }
-      if (RARE)
-#pragma unroll
-        for (int h = 0; h < NS; ++h) hidden(ks0 + 32 * h, s[h]);
     }
   };
   auto weights = [&]() {
@@ -822,11 +781,7 @@ __device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int k
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) vf[s2][dt] = __builtin_bit_cast(u32x4, tr_frag<W>(vt + h * SUB, 0, s2, dt, lane));
     __builtin_amdgcn_sched_barrier(0);
-    if (mask) {
-      const bool bad = not_finite<T, W>(vf);
-      rare |= bad;
-      if (RARE && bad) place_non_finite<T, W>(vf, st.o, st.lo - ks0 - 32 * h, st.hi - ks0 - 32 * h, hh);
-    }
+    if (mask) rare |= not_finite<T, W>(vf);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
       u32x4 pb;
@@ -895,31 +850,89 @@ __device__ __forceinline__ void load_row(const PagedAttnArgs& a, const FastArgs&
       for (int e = 0; e < 4; ++e) qf[ks][e] ^= 0x80008000u;
   }
 }
-// Keys of a subtile whose page does not exist.
-__device__ __forceinline__ void hide_missing(const PagedAttnArgs& a, const Tile& t, int ks0, int hh, f32x16& s) {
-  unsigned gone = 0u;
-#pragma unroll 1
-  for (int i = 0; i < 32; ++i) {
-    const int key = ks0 + i;
-    if (key >= t.khi || (unsigned)t.table[fast_div(key, a.by_page)] >= (unsigned)a.pages) gone |= 1u << i;
-  }
-  gone >>= 4 * hh;
+// The rows of a tile over keys [k0, k1) one by one, key by key: what a row does not see takes no part, whatever it holds.
+// For tiles with a missing page, or with a value that is not finite in a subtile that some row sees only in part, where a
+// product would carry 0 * inf into that row. Kept out of the common loops, whose registers it would spill. qs: LDS.
+template <typename T, int W>
+__device__ __forceinline__ void exact_rows(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, int slot, float* qs) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float c = f.negate ? -f.c : f.c;
+  float* const q_s = qs + wave * W;
+  for (int rr = wave; rr < t.nrows; rr += kThreads / 64) {
+    const int row = t.rows0 + rr;
+    const T* q = (const T*)a.q + row_offset(f, t, row, a.q_ts, a.q_hs);
+    const int pos = t.start + fast_div(row, f.by_group) + t.shift;
+    const int lo = max(k0, a.window > 0 ? max(pos - a.window + 1, 0) : 0), last = min(min(pos, t.cap - 1), k1 - 1);
+    for (int d = lane; d < W; d += 64) q_s[d] = d < a.width ? Cvt<T>::ld(q + d) : 0.f;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    float m = -INFINITY, l = 0.f, acc[W / 64];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) s[e] = gone & (1u << acc_row(e, 0)) ? -INFINITY : s[e];
+    for (int j = 0; j < W / 64; ++j) acc[j] = 0.f;
+    for (int key0 = lo; key0 <= last; key0 += 64) {
+      const int key = key0 + lane;
+      int pg = -1, in = 0;
+      if (key <= last) {
+        const int col = fast_div(key, a.by_page);
+        pg = t.table[col];
+        in = key - col * a.page;
+        if ((unsigned)pg >= (unsigned)a.pages) pg = -1;
+      }
+      float s = -INFINITY;
+      if (pg >= 0) {
+        const T* k = (const T*)a.k + pg * a.k_ps + in * a.k_rs + t.g * a.k_hs;
+        s = 0.f;
+        for (int d = 0; d < a.width; ++d) s += q_s[d] * Cvt<T>::ld(k + d);
+        s *= c;
+      }
+      const float to = fmaxf(m, wave_max(s)), base = to == -INFINITY ? 0.f : to;
+      const float p = pg >= 0 ? __builtin_amdgcn_exp2f(s - base) : 0.f, alpha = __builtin_amdgcn_exp2f(m - base);
+      l = l * alpha + wave_sum(p);
+      m = to;
+#pragma unroll
+      for (int j = 0; j < W / 64; ++j) acc[j] *= alpha;
+      for (int u = 0; u < 64; ++u) {
+        const int up = __shfl(pg, u, 64), ui = __shfl(in, u, 64);
+        const float pu = __shfl(p, u, 64);
+        if (up < 0) continue;
+        const T* v = (const T*)a.v + up * a.v_ps + ui * a.v_rs + t.g * a.v_hs;
+#pragma unroll
+        for (int j = 0; j < W / 64; ++j)
+          if (lane + 64 * j < a.width) acc[j] += pu * Cvt<T>::ld(v + lane + 64 * j);
+      }
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    if (slot >= 0) {
+      const long long at = (long long)slot * f.slot_rows + rr;
+#pragma unroll
+      for (int j = 0; j < W / 64; ++j) f.part[at * W + lane + 64 * j] = acc[j];
+      if (lane == 0) {
+        f.ml[at * 2] = m;
+        f.ml[at * 2 + 1] = l;
+      }
+    } else {
+      T* o = (T*)a.o + row_offset(f, t, row, a.o_ts, a.o_hs);
+#pragma unroll
+      for (int j = 0; j < W / 64; ++j)
+        if (lane + 64 * j < a.width) Cvt<T>::st(o + lane + 64 * j, l != 0.f ? acc[j] * inv : 0.f);
+    }
+  }
 }
 
-// One wave's subtiles of few rows: every fourth from ks0 on. Returns whether they need the RARE form.
-template <typename T, int W, bool UNI, bool RARE>
+// One wave's subtiles of few rows: every fourth from ks0 on. Returns whether they are a case for exact_rows().
+template <typename T, int W, int RUN>
 __device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int ks0, int k1, bool valid,
                                          char* kt, unsigned k_lds, int lane, u32x4 (&qf)[W / 16], RowState<W>& st) {
   constexpr int SUB = 32 * W * 2, NP = SUB / 1024;
   const int hh = lane >> 5;
   char* const vt = kt + SUB;
   const unsigned v_lds = k_lds + SUB;
-  PageRows<W, NP, UNI> pr;
+  PageRows<W, NP, RUN> pr;
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
   if (ks0 < k1) {
     pr.fetch(ks0);
+    pr.known(ks0);
     pr.template issue<false>(ks0, k_lds, f.stream);
     pr.template issue<true>(ks0, v_lds, f.stream);
   }
@@ -928,16 +941,18 @@ __device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs&
   for (; ks0 < k1; ks0 += kFewStep) {
     const int next = ks0 + kFewStep;
     const bool more = next < k1;
-    const bool gone = pr.gone;
-    const bool mask = gone || ks0 + 31 > t.p_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < t.p_last - a.window + 1);
+    rare |= pr.gone;
+    const bool mask = ks0 + 31 > t.p_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < t.p_last - a.window + 1);
     if (more) pr.fetch(next);
     wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
-    rare |= gone;
-    rare |= subtile<T, W, RARE>(
+    rare |= subtile<T, W>(
         kt, vt, ks0, mask, f.c, qf, st, lane,
         [&]() {
           wait_lds();         // the key fragments are in registers: their place takes the next subtile's
-          if (more) pr.template issue<false>(next, k_lds, f.stream);
+          if (more) {
+            pr.known(next);
+            pr.template issue<false>(next, k_lds, f.stream);
+          }
         },
         [&]() {
           if (more) wait_dma_but<NP>();
@@ -946,9 +961,6 @@ __device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs&
         [&]() {
           wait_lds();
           if (more) pr.template issue<true>(next, v_lds, f.stream);
-        },
-        [&](f32x16& s) {
-          if (gone) hide_missing(a, t, ks0, hh, s);
         });
   }
   return rare;
@@ -957,7 +969,7 @@ __device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs&
 // Few rows (at most 32) over keys [k0, k1), k0 a multiple of 32: subtile t belongs to wave t % 4, each wave has its own
 // part of LDS and its own running state; merged at the end, to the output (slot < 0) or to a slot of the workspace.
 // Leaves without a barrier behind its last reads of LDS.
-template <typename T, int W, bool UNI>
+template <typename T, int W, int RUN>
 __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, int slot,
                                          char* smem, unsigned lds0, float (&ml_s)[4][32][2]) {
   constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB;
@@ -971,15 +983,17 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs&
   u32x4 qf[W / 16];
   RowState<W> st;
   const bool valid = r32 < t.nrows;
-  if (few_loop<T, W, UNI, false>(a, f, t, k0 + wave * 32, k1, valid, kt, k_lds, lane, qf, st))
-    few_loop<T, W, UNI, true>(a, f, t, k0 + wave * 32, k1, valid, kt, k_lds, lane, qf, st);
+  const bool rare = few_loop<T, W, RUN>(a, f, t, k0 + wave * 32, k1, valid, kt, k_lds, lane, qf, st);
   // ---- merge the waves ----
   const float l = sum_halves(st.l);
   if (hh == 0) {
     ml_s[wave][r32][0] = st.mb;
     ml_s[wave][r32][1] = l;
   }
-  __syncthreads();
+  if (__syncthreads_or(rare)) {
+    exact_rows<T, W>(a, f, t, k0, k1, slot, reinterpret_cast<float*>(smem));
+    return;
+  }
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < 4; ++w)
@@ -1062,7 +1076,7 @@ __device__ __forceinline__ void write_meta(const FastArgs& f, int slot, int np, 
   m[6] = stride;
 }
 
-template <typename T, int W, bool UNI>
+template <typename T, int W, int RUN>
 __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kernel(PagedAttnArgs a, FastArgs f) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float ml_s[4][32][2];
@@ -1094,7 +1108,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kern
     const bool whole = s0 == 0 && s1 == steps;
     const int slot = whole ? -1 : 2 * id + (first_run ? 0 : 1);
     if (!first_run) __syncthreads();                  // the last run's outputs have been read from LDS
-    few_rows<T, W, UNI>(a, f, t, k0, k1, slot, smem, lds0, ml_s);
+    few_rows<T, W, RUN>(a, f, t, k0, k1, slot, smem, lds0, ml_s);
     if (!whole && s0 == 0 && tid == 0) {
       const int last = (at + steps - 1) / per;        // the workgroup that has its end
       write_meta(f, slot, last - id + 1, t.start, rows0, t.nrows, g, 2 * id, 2);
@@ -1103,19 +1117,21 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kern
   }
 }
 
-// 128 rows over keys [k0, k1), k0 a multiple of 64: the waves share 64-key tiles. Returns whether the RARE form is needed.
-template <typename T, int W, bool UNI, bool RARE>
-__device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1, bool missing,
+// 128 rows over keys [k0, k1), k0 a multiple of 64: the waves share 64-key tiles. Returns whether they are a case for
+// exact_rows().
+template <typename T, int W, int RUN>
+__device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1,
                                            char* smem, unsigned lds0, int wave, int lane, u32x4 (&qf)[W / 16], RowState<W>& st) {
   constexpr int SUB = 32 * W * 2, NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;   // transfers per wave and tile; a K and a V tile
   constexpr int NS = DPA_NS;
   const int r32 = lane & 31, hh = lane >> 5;
-  PageRows<W, NP, UNI> pr;
+  PageRows<W, NP, RUN> pr;
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
   const int w_off = wave * 16;                               // the 16 rows of a tile that the wave transfers
   const unsigned w_lds = lds0 + wave * NP * 1024;
   if (k0 < k1) {
     pr.fetch(k0 + w_off);
+    pr.known(k0 + w_off);
     pr.template issue<false>(k0 + w_off, w_lds);
     pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
   }
@@ -1126,16 +1142,17 @@ __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArg
   const bool wave_live = row < t.rows;
   bool rare = false;
   int stage = 0;
-  if (k0 + 64 < k1) pr.fetch(k0 + 64 + w_off);
   for (int kt0 = k0; kt0 < k1; kt0 += 64) {
+    const int next = kt0 + 64;
+    rare |= pr.gone;                            // of this tile
+    if (next < k1) pr.fetch(next + w_off);      // (under the wait for this tile)
     wait_dma_but<0>();
     __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
-    const int next = kt0 + 64;
     if (next < k1) {
       const unsigned nb = w_lds + (stage ^ 1) * STAGE;
+      pr.known(next + w_off);
       pr.template issue<false>(next + w_off, nb);
       pr.template issue<true>(next + w_off, nb + 2 * SUB);
-      if (next + 64 < k1) pr.fetch(next + 64 + w_off);
     }
     const char* const kt = smem + stage * STAGE;
     const char* const vt = kt + 2 * SUB;
@@ -1145,19 +1162,17 @@ __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArg
     for (int ks0 = kt0; ks0 < kt0 + 64; ks0 += 32 * NS) {
       if (ks0 > wp_last || ks0 >= t.khi) break;
       if (a.window > 0 && ks0 + 32 * NS - 1 < wp_first - a.window + 1) continue;
-      const bool mask = missing || ks0 + 32 * NS - 1 > wp_first || ks0 + 32 * NS > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
+      const bool mask = ks0 + 32 * NS - 1 > wp_first || ks0 + 32 * NS > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
       const int at = (ks0 - kt0) * W * 2;
-      rare |= chunk_tile<T, W, NS, RARE>(kt + at, vt + at, ks0, mask, f.c, qf, st, lane, [&](int k, f32x16& s) {
-        if (missing) hide_missing(a, t, k, hh, s);
-      });
+      rare |= chunk_tile<T, W, NS>(kt + at, vt + at, ks0, mask, f.c, qf, st, lane);
     }
   }
   return rare;
 }
 
 // Chunks, with few-row requests among them.
-template <typename T, int W, bool UNI>
-__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
+template <typename T, int W, int RUN>
+__global__ __launch_bounds__(kThreads, DPA_LB) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
   constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float ml_s[4][32][2];
@@ -1187,25 +1202,18 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(P
   const int k0 = k_base + piece * span, k1 = min(t.khi, k0 + span);
   if (np > 1 && tid == 0) write_meta(f, slot, piece == 0 ? np : 0, q.start, rows0, nrows, g, slot, a.nkv);
   if (!q.chunk) {
-    few_rows<T, W, UNI>(a, f, t, k0, k1, np > 1 ? slot : -1, smem, lds0, ml_s);
+    few_rows<T, W, RUN>(a, f, t, k0, k1, np > 1 ? slot : -1, smem, lds0, ml_s);
     return;
   }
 
-  // ---- a chunk: do all pages of the piece exist? ----
-  bool missing = false;
-  if (k1 > k0) {
-    const int c_lo = fast_div(max(k0, t.klo), a.by_page), c_hi = fast_div(k1 - 1, a.by_page);
-    for (int col = c_lo + tid; col <= c_hi; col += kThreads) missing |= (unsigned)t.table[col] >= (unsigned)a.pages;
-  }
-  missing = __syncthreads_or(missing);
-
   u32x4 qf[W / 16];
   RowState<W> st;
-  bool rare = missing;
-  if (!rare) rare = __syncthreads_or(chunk_loop<T, W, UNI, false>(a, f, t, k0, k1, false, smem, lds0, wave, lane, qf, st));
-  if (rare) chunk_loop<T, W, UNI, true>(a, f, t, k0, k1, missing, smem, lds0, wave, lane, qf, st);
+  // (a barrier too: every wave is done with the tiles)
+  if (__syncthreads_or(chunk_loop<T, W, RUN>(a, f, t, k0, k1, smem, lds0, wave, lane, qf, st))) {
+    exact_rows<T, W>(a, f, t, k0, k1, np > 1 ? slot : -1, reinterpret_cast<float*>(smem));
+    return;
+  }
   const float l = sum_halves(st.l);
-  __syncthreads();          // every wave is done with the tiles
   char* const tile_o = smem + wave * REGION;
   const float inv = np > 1 ? 1.f : (l != 0.f ? 1.f / l : 0.f);
 #pragma unroll
@@ -1314,7 +1322,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs
   *reinterpret_cast<u32x4*>((uint16_t*)a.o + (long long)(start + tk) * a.o_ts + (long long)hd * a.o_hs + 8 * d8) = w;
 }
 
-// Whether the matrix kernels take the call: 16-bit types, whole aligned 16-byte pieces, offsets inside a page below 2^32.
+// Whether the matrix kernels take the call: 16-bit types, whole aligned 16-byte pieces, offsets inside a page below 2^31.
 bool fast_ok(const PagedAttnArgs& a) {
   if (a.type == kTypeFloat || a.width % 8 != 0 || a.width > 128) return false;
   const long long strides[] = {a.q_ts, a.q_hs, a.o_ts, a.o_hs, a.k_ps, a.k_rs, a.k_hs, a.v_ps, a.v_rs, a.v_hs};
@@ -1323,7 +1331,7 @@ bool fast_ok(const PagedAttnArgs& a) {
   for (const void* p : {a.q, a.k, a.v, (const void*)a.o})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
   const long long lim = 1ll << 31;
-  return a.k_rs * 2 * std::max(a.page, 8) < lim && a.v_rs * 2 * std::max(a.page, 8) < lim;
+  return a.k_rs * 2 * std::max(a.page, 16) < lim && a.v_rs * 2 * std::max(a.page, 16) < lim && a.k_ps * 2 < lim && a.v_ps * 2 < lim;
 }
 
 struct Plan {
@@ -1336,7 +1344,7 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
   p.chunks = (long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows;
   if (p.chunks) {
-    p.target = num_cus * 4;
+    p.target = num_cus * DPA_T;
     // tiles: one per request with rows, and one more for every 128 rows of a chunk
     const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
     p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
@@ -1356,10 +1364,10 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   return p;
 }
 
-template <typename T, int W, bool UNI, bool CHUNKS>
+template <typename T, int W, int RUN, bool CHUNKS>
 void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
   constexpr int lds = 4 * 2 * 32 * W * 2;
-  auto kernel = CHUNKS ? paged_attn_kernel<T, W, UNI> : paged_attn_few_kernel<T, W, UNI>;
+  auto kernel = CHUNKS ? paged_attn_kernel<T, W, RUN> : paged_attn_few_kernel<T, W, RUN>;
   static bool set = false;       // above the default limit of dynamic LDS; the same value every time
   if (!set) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -1372,11 +1380,16 @@ void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_
 }
 template <typename T, int W>
 void launch_fast(const PagedAttnArgs& a, const FastArgs& f, const Plan& p, hipStream_t st) {
-  const bool uni = a.width == W && a.page % (512 / W) == 0;      // a 1 KiB transfer lies in one page
-  if (uni && p.chunks) launch_fast<T, W, true, true>(a, f, p.grid, st);
-  else if (uni) launch_fast<T, W, true, false>(a, f, p.grid, st);
-  else if (p.chunks) launch_fast<T, W, false, true>(a, f, p.grid, st);
-  else launch_fast<T, W, false, false>(a, f, p.grid, st);
+  const int run = a.width != W ? 0 : a.page % 16 == 0 ? 16 : a.page % (512 / W) == 0 ? 512 / W : 0;
+  if (p.chunks) {
+    if (run == 16) launch_fast<T, W, 16, true>(a, f, p.grid, st);
+    else if (run > 0) launch_fast<T, W, 512 / W, true>(a, f, p.grid, st);
+    else launch_fast<T, W, 0, true>(a, f, p.grid, st);
+  } else {
+    if (run == 16) launch_fast<T, W, 16, false>(a, f, p.grid, st);
+    else if (run > 0) launch_fast<T, W, 512 / W, false>(a, f, p.grid, st);
+    else launch_fast<T, W, 0, false>(a, f, p.grid, st);
+  }
 }
 
 }  // namespace

@@ -262,16 +262,18 @@ def test_attention_values_in_masked_places_stay_there(n, window, width, bad):
     cu, kv = i32(0, n), i32(L)
     at = L - 1 - n // 2              # the position of the row in the middle
     slot = int(table[0, at // 16]) * 16 + at % 16
-    clean = ops.paged_attention(q, k, v, table, cu, kv, window=window)
     v.view(-1, 2, width)[slot, :, 3] = bad
     o = ops.paged_attention(q, k, v, table, cu, kv, window=window)
     pos = torch.arange(L - n, L, device=DEV)
     sees = pos >= at
     if window:
         sees &= pos < at + window
-    assert torch.equal(o[~sees], clean[~sees]) and not torch.isfinite(o[sees][:, :, 3]).any()
+    assert not torch.isfinite(o[sees][:, :, 3]).any()
     rest = [d for d in range(width) if d != 3]
-    assert torch.equal(o[..., rest], clean[..., rest])
+    # elsewhere what the clean values give, within the formula's roundings: such tiles may be summed in another order
+    want, tol = bound(q, k, torch.nan_to_num(v, 0.0, 0.0, 0.0), table, cu, kv, 1 / math.sqrt(width), window, L)
+    assert ((o[~sees].double() - want[~sees]).abs() <= tol[~sees]).all()
+    assert ((o[..., rest].double() - want[..., rest]).abs() <= tol[..., rest]).all()
     v.view(-1, 2, width)[slot, :, 3] = 0
     k.view(-1, 2, width)[slot] = math.nan
     o = ops.paged_attention(q, k, v, table, cu, kv, window=window)
