@@ -1,12 +1,3 @@
-#ifndef DPA_NS
-#define DPA_NS (W == 64 ? 1 : 2)
-#endif
-#ifndef DPA_T
-#define DPA_T 2
-#endif
-#ifndef DPA_LB
-#define DPA_LB (W==64?3:2)
-#endif
 // Causal attention of the newest tokens of every request over its pages (gfx950). Row i of request r sits at position
 // pos = kv[r] - n[r] + i - cu[r] (n[r] = cu[r + 1] - cu[r]) and attends keys max(0, pos - window + 1) .. pos:
 //
@@ -523,72 +514,87 @@ struct PageRows {
       kv_off[1][v] = (unsigned)in_run * (unsigned)(2 * args.v_rs) + col;
     }
   }
-  __device__ __forceinline__ bool whole(int ks0) const { return RUN > 0 && ks0 >= klo && ks0 + NP * RPP <= khi; }
+  // Every row exists and somebody may see it: all lanes transfer, and a transfer is one instruction per piece.
+  __device__ __forceinline__ bool whole(int ks0) const { return RUN > 0 && !gone && ks0 >= klo && ks0 + NP * RPP <= khi; }
   // page numbers of the rows [ks0, ks0 + NP * RPP), for the issue() of those rows; known() waits for them
   __device__ __forceinline__ void fetch(int ks0) {
-    if (whole(ks0)) {
+    if constexpr (RUN > 0) {
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const int col = fast_div(ks0 + i * PER * RPP, a->by_page);
+        const int col = fast_div(min(ks0 + i * RUN, khi - 1), a->by_page);
         typedef const __attribute__((address_space(4))) int* scalar_ptr;
         pg[i] = *(scalar_ptr)(unsigned long long)(table + __builtin_amdgcn_readfirstlane(col));
       }
-    } else if (RUN == 0) {
+    } else {
 #pragma unroll
-      for (int pc = 0; pc < NP; ++pc) pg[pc] = lane_page(ks0 + pc * RPP + lane / CPR);
+      for (int pc = 0; pc < NP; ++pc) {
+        const int key = ks0 + pc * RPP + lane / CPR;
+        pg[pc] = key >= klo && key < khi ? table[fast_div(key, a->by_page)] : -1;
+      }
     }
   }
   __device__ __forceinline__ void known(int ks0) {
     bool bad = false;
-    if (whole(ks0)) {
+    if constexpr (RUN > 0) {
 #pragma unroll
-      for (int i = 0; i < NR; ++i) bad |= (unsigned)pg[i] >= (unsigned)a->pages;
+      for (int i = 0; i < NR; ++i) {
+        const int r0 = ks0 + i * RUN;
+        bad |= r0 < khi && r0 + RUN > klo && (unsigned)pg[i] >= (unsigned)a->pages;
+      }
     } else {
 #pragma unroll
       for (int pc = 0; pc < NP; ++pc) {
-        const int key = ks0 + pc * RPP + lane / CPR, p = RUN == 0 ? pg[pc] : lane_page(key);
-        bad |= key >= klo && key < khi && (unsigned)p >= (unsigned)a->pages;
+        const int key = ks0 + pc * RPP + lane / CPR;
+        bad |= key >= klo && key < khi && (unsigned)pg[pc] >= (unsigned)a->pages;
       }
       bad = __any(bad);
     }
     gone = bad;
   }
-  __device__ __forceinline__ int lane_page(int key) const {
-    return key >= klo && key < khi ? table[fast_div(key, a->by_page)] : -1;
-  }
-  // `stream` (few rows over pools past the memory-side cache: every byte is read once): without a place in the caches
+  // `stream` (few rows over pools past the memory-side cache: every byte is read once): without a place in the caches.
+  // Rows that no query may see, and rows of missing pages, become zeros.
   template <bool V>
   __device__ __forceinline__ void issue(int ks0, unsigned lds, bool stream = false) const {
     const unsigned long long base = V ? vb : kb;
     const unsigned ps = 2u * (unsigned)(V ? a->v_ps : a->k_ps), rs = 2u * (unsigned)(V ? a->v_rs : a->k_rs);
-    if (whole(ks0) && !gone) {
+    if constexpr (RUN > 0) {
       unsigned long long from[NR];
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const int key = ks0 + i * PER * RPP;
-        const unsigned row = __builtin_amdgcn_readfirstlane(key - fast_div(key, a->by_page) * a->page);
+        const int key = min(ks0 + i * RUN, khi - 1);
+        const unsigned row = __builtin_amdgcn_readfirstlane(key - fast_div(key, a->by_page) * a->page) & ~(RUN - 1);
         const unsigned p = __builtin_amdgcn_readfirstlane(pg[i]);
         from[i] = base + (unsigned long long)p * ps + row * rs;
       }
-      if (stream) {
+      if (whole(ks0)) {
+        if (stream) {
 #pragma unroll
-        for (int pc = 0; pc < NP; ++pc) dma_uniform<true>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);
-      } else {
+          for (int pc = 0; pc < NP; ++pc) dma_uniform<true>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);
+        } else {
 #pragma unroll
-        for (int pc = 0; pc < NP; ++pc) dma_uniform<false>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);
+          for (int pc = 0; pc < NP; ++pc) dma_uniform<false>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);
+        }
+        return;
       }
-      return;
-    }
 #pragma unroll
-    for (int pc = 0; pc < NP; ++pc) {
-      const int row = pc * RPP + lane / CPR, key = ks0 + row;
-      const int ch = swz<W>(row, lane % CPR);
-      unsigned long long addr = (unsigned long long)zero_row + 16u * ch;
-      const int p = RUN == 0 ? pg[pc] : lane_page(key);
-      const int col = fast_div(max(key, 0), a->by_page);
-      if ((unsigned)p < (unsigned)a->pages && key >= klo && key < khi && ch * 8 < a->width)
-        addr = base + (unsigned long long)(unsigned)p * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
-      dma_lane(addr, lds + pc * 1024);
+      for (int pc = 0; pc < NP; ++pc) {
+        const int key = ks0 + pc * RPP + lane / CPR;
+        if ((unsigned)pg[pc / PER] < (unsigned)a->pages && key >= klo && key < khi)
+          dma_uniform<false>(from[pc / PER], kv_off[V][pc % OFF], lds + pc * 1024);    // (lanes that are off leave their place alone)
+        else
+          *(__attribute__((address_space(3))) u32x4*)(size_t)(lds + pc * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+      }
+    } else {
+#pragma unroll
+      for (int pc = 0; pc < NP; ++pc) {
+        const int row = pc * RPP + lane / CPR, key = ks0 + row;
+        const int ch = swz<W>(row, lane % CPR), p = pg[pc];
+        unsigned long long addr = (unsigned long long)zero_row + 16u * ch;
+        const int col = fast_div(max(key, 0), a->by_page);
+        if ((unsigned)p < (unsigned)a->pages && ch * 8 < a->width)      // (-1: nobody sees the row)
+          addr = base + (unsigned long long)(unsigned)p * ps + (unsigned)(key - col * a->page) * rs + 16u * ch;
+        dma_lane(addr, lds + pc * 1024);
+      }
     }
   }
 };
@@ -849,6 +855,10 @@ __device__ __forceinline__ void load_row(const PagedAttnArgs& a, const FastArgs&
 #pragma unroll
       for (int e = 0; e < 4; ++e) qf[ks][e] ^= 0x80008000u;
   }
+  // Have them here: their first use is inside the caller's loop, where the compiler's wait for them would, in every
+  // round, wait for the transfers of the next tile as well.
+#pragma unroll
+  for (int ks = 0; ks < W / 16; ++ks) asm volatile("" : "+v"(qf[ks]));
 }
 // The rows of a tile over keys [k0, k1) one by one, key by key: what a row does not see takes no part, whatever it holds.
 // For tiles with a missing page, or with a value that is not finite in a subtile that some row sees only in part, where a
@@ -930,9 +940,11 @@ __device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs&
   const unsigned v_lds = k_lds + SUB;
   PageRows<W, NP, RUN> pr;
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
+  bool partial = false;       // the subtile whose transfer was begun last
   if (ks0 < k1) {
     pr.fetch(ks0);
     pr.known(ks0);
+    partial = !pr.whole(ks0);
     pr.template issue<false>(ks0, k_lds, f.stream);
     pr.template issue<true>(ks0, v_lds, f.stream);
   }
@@ -944,18 +956,22 @@ __device__ __forceinline__ bool few_loop(const PagedAttnArgs& a, const FastArgs&
     rare |= pr.gone;
     const bool mask = ks0 + 31 > t.p_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < t.p_last - a.window + 1);
     if (more) pr.fetch(next);
-    wait_dma_but<NP>();       // the keys of this subtile are in LDS, its values may be on their way
+    // the keys of this subtile are in LDS, its values may be on their way (as one instruction per piece, if it is whole)
+    const bool whole = RUN == 0 || !partial;
+    if (whole) wait_dma_but<NP>();
+    else wait_dma_but<0>();
     rare |= subtile<T, W>(
         kt, vt, ks0, mask, f.c, qf, st, lane,
         [&]() {
           wait_lds();         // the key fragments are in registers: their place takes the next subtile's
           if (more) {
             pr.known(next);
+            partial = !pr.whole(next);
             pr.template issue<false>(next, k_lds, f.stream);
           }
         },
         [&]() {
-          if (more) wait_dma_but<NP>();
+          if (more && (RUN == 0 || !partial)) wait_dma_but<NP>();
           else wait_dma_but<0>();
         },
         [&]() {
@@ -1123,7 +1139,7 @@ template <typename T, int W, int RUN>
 __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1,
                                            char* smem, unsigned lds0, int wave, int lane, u32x4 (&qf)[W / 16], RowState<W>& st) {
   constexpr int SUB = 32 * W * 2, NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;   // transfers per wave and tile; a K and a V tile
-  constexpr int NS = DPA_NS;
+  constexpr int NS = 1;       // subtiles taken together; 2: 668 instead of 653 us on the 16k prefill (fewer registers to schedule with)
   const int r32 = lane & 31, hh = lane >> 5;
   PageRows<W, NP, RUN> pr;
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
@@ -1172,7 +1188,7 @@ __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArg
 
 // Chunks, with few-row requests among them.
 template <typename T, int W, int RUN>
-__global__ __launch_bounds__(kThreads, DPA_LB) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
+__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
   constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float ml_s[4][32][2];
@@ -1344,7 +1360,7 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
   p.chunks = (long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows;
   if (p.chunks) {
-    p.target = num_cus * DPA_T;
+    p.target = num_cus * 2;
     // tiles: one per request with rows, and one more for every 128 rows of a chunk
     const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
     p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
