@@ -198,7 +198,8 @@ __device__ __forceinline__ Request request(const PagedAttnArgs& a, const FastArg
   return q;
 }
 
-// Work of a request in keys walked by a workgroup: a 64-key step of a chunk takes as long as a 128-key one of few rows.
+// Work of a request: keys walked by a workgroup, those of a chunk counted twice (its steps have 64 keys, those of few
+// rows 128).
 __device__ __forceinline__ float request_cost(const Request& q) {
   return (float)q.tiles * (float)(q.khi - q.klo) * (q.chunk ? 2.f : 1.f);
 }
@@ -331,7 +332,7 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
 // A (request, 32 packed rows, KV head) is a run of 128-key steps (one at least); the runs lie one after another, and workgroup i of `eff`
 // takes steps [i * per, (i + 1) * per) of them all, whichever runs they fall into: contexts of any mix of lengths load
 // the card evenly in one round. At most its first and its last run are cut.
-constexpr int kMinSteps = 2;           // fewer steps than this are not worth a workgroup of their own
+constexpr int kMinSteps = 1;           // fewer steps than this are not worth a workgroup of their own
 __device__ __forceinline__ int run_base(const Request& q) { return q.klo & ~31; }
 __device__ __forceinline__ int run_steps(const Request& q) {
   return q.rows > 0 ? max((q.khi - run_base(q) + kFewStep - 1) / kFewStep, 1) : 0;
@@ -1145,31 +1146,29 @@ __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArg
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
   const int w_off = wave * 16;                               // the 16 rows of a tile that the wave transfers
   const unsigned w_lds = lds0 + wave * NP * 1024;
+  bool rare = false;
+  auto request_tile = [&](int at, int stage) {
+    pr.known(at + w_off);
+    rare |= pr.gone;
+    pr.template issue<false>(at + w_off, w_lds + stage * STAGE);
+    pr.template issue<true>(at + w_off, w_lds + stage * STAGE + 2 * SUB);
+  };
   if (k0 < k1) {
     pr.fetch(k0 + w_off);
-    pr.known(k0 + w_off);
-    pr.template issue<false>(k0 + w_off, w_lds);
-    pr.template issue<true>(k0 + w_off, w_lds + 2 * SUB);
+    request_tile(k0, 0);
   }
   const int row = t.rows0 + wave * 32;
   load_row<W>(a, f, t, row + r32, row + r32 < t.rows, hh, qf, st);
   const int wp_first = t.start + fast_div(min(row, t.rows - 1), f.by_group) + t.shift;
   const int wp_last = t.start + fast_div(min(row + 31, t.rows - 1), f.by_group) + t.shift;
   const bool wave_live = row < t.rows;
-  bool rare = false;
   int stage = 0;
   for (int kt0 = k0; kt0 < k1; kt0 += 64) {
     const int next = kt0 + 64;
-    rare |= pr.gone;                            // of this tile
     if (next < k1) pr.fetch(next + w_off);      // (under the wait for this tile)
     wait_dma_but<0>();
     __syncthreads();        // the tile has landed for every wave; every wave is done with the other stage
-    if (next < k1) {
-      const unsigned nb = w_lds + (stage ^ 1) * STAGE;
-      pr.known(next + w_off);
-      pr.template issue<false>(next + w_off, nb);
-      pr.template issue<true>(next + w_off, nb + 2 * SUB);
-    }
+    if (next < k1) request_tile(next, stage ^ 1);      // (two ahead, in a third stage: no difference)
     const char* const kt = smem + stage * STAGE;
     const char* const vt = kt + 2 * SUB;
     stage ^= 1;
