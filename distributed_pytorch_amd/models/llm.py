@@ -25,7 +25,8 @@ What is different underneath:
   round trips, no expert loop); the aux-free bias is updated exactly once per training forward,
   also under activation recomputation; attention dropout runs inside the flash kernels;
 * cached decoding uses a bottom-right aligned causal mask (the reference's GQA path attends to
-  key 0 only when decoding from a cache).
+  key 0 only when decoding from a cache); requests of different lengths generate as one packed batch
+  over a paged cache (``generate_ragged``).
 """
 from __future__ import annotations
 
@@ -42,7 +43,7 @@ from torch.utils.checkpoint import checkpoint
 from .. import ops
 from ..config import LLMconfig
 
-__all__ = ["LLM", "Block", "GQA", "NaiveMHLA", "FullMHLA", "Attention", "MLP", "Expert", "MoE"]
+__all__ = ["LLM", "PagedKVCache", "Block", "GQA", "NaiveMHLA", "FullMHLA", "Attention", "MLP", "Expert", "MoE"]
 
 _tls = threading.local()
 
@@ -134,6 +135,50 @@ class _StaticLayer:
         self.k, self.v, self.pos, self.len_after = k, v, pos, len_after
 
 
+class PagedKVCache:
+    """Key / value cache of a ragged batch: requests of different lengths, pages handed out as they grow (GQA family).
+
+    Per layer a pool ``k[i], v[i] [pages, page_size, n_kv_heads, head_size]``; the table, the lengths and the free list
+    are device tensors (``ops/paged.py``), so a step has no host-side shape but its number of rows and can be captured.
+    A step: ``begin(q_lens, num_tokens)``, a forward of the packed tokens ``[1, num_tokens]``, ``commit()``."""
+
+    def __init__(self, config: LLMconfig, requests: int, max_len: int, pages: int, device, dtype, page_size: int = 16):
+        if config.attn not in ("mha", "mqa", "gqa"):
+            raise ValueError("the paged cache holds key / value heads: no latent attention")
+        if max_len > config.block_size:
+            raise ValueError(f"max_len {max_len} exceeds the context of {config.block_size} positions")
+        shape = (pages, page_size, config.n_kv_heads, config.n_embd // config.n_head)
+        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(config.n_layer)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(config.n_layer)]
+        self.page_size = page_size
+        columns = (max_len + page_size - 1) // page_size
+        self.table = torch.full((requests, columns), -1, dtype=torch.int32, device=device)
+        self.ctx_lens = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(pages, dtype=torch.int32, device=device)
+        self.free_left = torch.tensor([pages, 0], dtype=torch.int32, device=device)   # [1]: pages a step asked for in vain
+        self.plan = None
+        self.max_q = None
+
+    def begin(self, q_lens: torch.Tensor, num_tokens: int, max_q: int | None = None):
+        """Pages and slots for ``q_lens`` (int32 ``[requests]``) new tokens; ``max_q``: the host's bound of them."""
+        self.plan = ops.paged_plan(q_lens, self.ctx_lens, self.table, self.free_pages, self.free_left, self.page_size, num_tokens)
+        self.max_q = max_q
+
+    def commit(self):
+        self.ctx_lens.copy_(self.plan.kv_lens)
+        self.free_left.copy_(self.plan.free_left)
+
+    def layer(self, i: int):
+        return _PagedLayer(self.k[i], self.v[i], self)
+
+
+class _PagedLayer:
+    __slots__ = ("k", "v", "cache")
+
+    def __init__(self, k, v, cache):
+        self.k, self.v, self.cache = k, v, cache
+
+
 # ---------------------------------------------------------------------------------------------
 class GQA(nn.Module):
     """Grouped-query attention (MHA / MQA / GQA) with or without RoPE
@@ -178,6 +223,13 @@ class GQA(nn.Module):
             q, k, v = ops.split_qkv(qkv, nh, nkv)
             ops.kv_append(kv_cache.k, kv_cache.v, k, v, kv_cache.pos)
             y = ops.cached_attention(q, kv_cache.k, kv_cache.v, kv_cache.len_after)
+            new_cache = kv_cache
+        elif isinstance(kv_cache, _PagedLayer):
+            # packed tokens of all requests: their rows into the pages, attention of each over its own
+            q, k, v = ops.split_qkv(qkv, nh, nkv)
+            cache, plan = kv_cache.cache, kv_cache.cache.plan
+            ops.paged_append(kv_cache.k, kv_cache.v, k[0], v[0], plan.slots)
+            y = ops.paged_attention(q[0], kv_cache.k, kv_cache.v, cache.table, plan.cu_q, plan.kv_lens, max_q=cache.max_q)
             new_cache = kv_cache
         elif kv_cache is None and not self._want_cache():
             y = ops.causal_self_attention_qkv(qkv, nh, nkv, dropout_p=p_drop)
@@ -792,6 +844,7 @@ class LLM(nn.Module):
         cfg = self.config
         B, T = idx.shape
         wte = self.lm_head.weight
+        paged = None
         if isinstance(kv_caches, StaticKVCache):
             # decode step over the preallocated cache: the position is a device scalar, so the position
             # row / rotary rows are gathered on the device and handed to the kernels as 1-row tables
@@ -803,6 +856,17 @@ class LLM(nn.Module):
             if cfg.pos_emb == "rope":
                 rope = (self.rope_cos.index_select(0, static.pos), self.rope_sin.index_select(0, static.pos), 0)
             kv_caches = [static.layer(i) for i in range(cfg.n_layer)]
+        elif isinstance(kv_caches, PagedKVCache):
+            # packed tokens of a ragged batch: every row has a position of its own, gathered on the device
+            assert B == 1 and targets is None, "paged cache: the requests' tokens in one row, no targets"
+            paged = kv_caches
+            at = paged.plan.positions
+            ptab = self._pos_table(wte.dtype, wte.device)
+            x = ops.embedding(idx, wte, None if ptab is None else ptab.index_select(0, at), 0)
+            rope = None
+            if cfg.pos_emb == "rope":
+                rope = (self.rope_cos.index_select(0, at), self.rope_sin.index_select(0, at), 0)
+            kv_caches = [paged.layer(i) for i in range(cfg.n_layer)]
         else:
             start_pos = self._start_pos(kv_caches)
             x = ops.embedding(idx, wte, self._pos_table(wte.dtype, wte.device), start_pos)
@@ -852,6 +916,11 @@ class LLM(nn.Module):
                 main_loss = ops.linear_cross_entropy(x, wte, targets, chunk_rows=self.loss_chunk_rows,
                                                      expected_grad=self.loss_grad_scale if self.training else 1.0)
             loss = main_loss + total_aux / cfg.n_layer
+        elif paged is not None:
+            # the newest row of every request: logits [requests, 1, V]
+            last = (paged.plan.cu_q[1:] - 1).clamp_(min=0)
+            logits = ops.linear(x[0].index_select(0, last)[:, None, :], wte)
+            loss = None
         else:
             logits = ops.linear(x[:, -1:, :], wte)   # a slice, not a list index: no host-built index tensor
             loss = None
@@ -868,13 +937,16 @@ class LLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature: float = 1.0, topk: int | None = None,
-                 hip_graph: bool | None = None):
+                 hip_graph: bool | None = None, penalties: dict | None = None):
         """KV-cache sampling with a sliding window of ``block_size - 1`` cached positions
         (reference: single-gpu/model.py:699-747).
 
         ``hip_graph`` (default: automatic) decodes from ONE captured hipGraph per token over a
         preallocated cache when the model is on the GPU, its key rows fit the flash kernels (head size
-        64 / 128, or an MLA latent key of at most 128 columns) and prompt plus new tokens fit the context: a decode step is a few hundred small kernels, bound by launch cost."""
+        64 / 128, or an MLA latent key of at most 128 columns) and prompt plus new tokens fit the context: a decode step is a few hundred small kernels, bound by launch cost.
+
+        ``penalties``: keyword arguments of ``ops.penalize_logits`` (``repetition``, ``presence``, ``frequency``, ``bias``,
+        ``allowed``), applied to the logits of every step with the tokens so far as the history."""
         was_training = self.training
         self.eval()
         try:
@@ -885,16 +957,16 @@ class LLM(nn.Module):
                 hip_graph = able
             self.last_decode_graphed = False      # introspection: did the last call replay a graph?
             if hip_graph and able:
-                out = self._generate_graphed(idx, max_new_tokens, temperature, topk)
+                out = self._generate_graphed(idx, max_new_tokens, temperature, topk, penalties)
                 if out is not None:
                     self.last_decode_graphed = True
                     return out
-            return self._generate_eager(idx, max_new_tokens, temperature, topk)
+            return self._generate_eager(idx, max_new_tokens, temperature, topk, penalties)
         finally:
             if was_training:
                 self.train()
 
-    def _generate_graphed(self, idx, max_new_tokens, temperature, topk):
+    def _generate_graphed(self, idx, max_new_tokens, temperature, topk, penalties=None):
         """Prompt through the normal forward, then one eager decode step over the static cache (lazy
         initialisations happen outside the capture), then the same step captured once and replayed for
         every remaining token. Returns None if the step cannot be captured."""
@@ -905,8 +977,18 @@ class LLM(nn.Module):
         static = StaticKVCache(cfg, B, cfg.block_size, dev, self.lm_head.weight.dtype)
         static.fill(caches, P)
         del caches
-        out = torch.empty(B, max_new_tokens, dtype=torch.int64, device=dev)
-        tok = self._sample(logits, temperature, topk)
+        history = torch.empty(B, P + max_new_tokens, dtype=torch.int64, device=dev)
+        history[:, :P] = idx
+        out = history[:, P:]
+        prompt_len = torch.full((1,), P, dtype=torch.int32, device=dev)
+
+        def penalize(lg, total):
+            """The logits ``[B, 1, V]`` with the penalties for the first ``total`` (int32 [1]) tokens of the history."""
+            if not penalties:
+                return lg
+            return ops.penalize_logits(lg[:, -1, :], history, prompt_len, total, **penalties)[:, None, :]
+
+        tok = self._sample(penalize(logits, prompt_len), temperature, topk)
         out[:, :1] = tok
         out_pos = torch.ones(1, dtype=torch.int64, device=dev)
 
@@ -918,6 +1000,7 @@ class LLM(nn.Module):
 
         def step():
             lg, _, _ = self.forward(tok, kv_caches=static)
+            lg = penalize(lg, static.len_after)
             if one_launch:
                 # sampling, history write, next input and the counter updates in the sampler's launch
                 ops.sample_step(lg[:, -1, :], temperature, topk, seed, tok, out, out_pos, static.pos, static.len_after, ticket)
@@ -940,10 +1023,11 @@ class LLM(nn.Module):
             return None
         for _ in range(max_new_tokens - 2):
             graph.replay()
-        return torch.cat((idx, out), dim=1)
+        return history
 
-    def _generate_eager(self, idx, max_new_tokens, temperature, topk):
+    def _generate_eager(self, idx, max_new_tokens, temperature, topk, penalties=None):
         cfg = self.config
+        prompt_len = torch.full((1,), idx.size(1), dtype=torch.int32, device=idx.device)
         kv_caches = [None] * cfg.n_layer
         for i in range(max_new_tokens):
             inp = (idx if idx.size(1) <= cfg.block_size else idx[:, -cfg.block_size:]) if i == 0 else idx[:, -1:]
@@ -958,5 +1042,70 @@ class LLM(nn.Module):
                     else:
                         kv_caches[li] = c[:, -keep:, :]
             logits, _, kv_caches = self.forward(inp, kv_caches=kv_caches)
+            if penalties:
+                logits = ops.penalize_logits(logits[:, -1, :], idx, prompt_len, **penalties)[:, None, :]
             idx = torch.cat((idx, self._sample(logits, temperature, topk)), dim=1)
         return idx
+
+    @torch.no_grad()
+    def generate_ragged(self, prompts, max_new_tokens: int, temperature: float = 1.0, topk: int | None = None,
+                        hip_graph: bool | None = None, penalties: dict | None = None, page_size: int = 16):
+        """Sampling for prompts of different lengths in one batch: ``prompts`` (a list of 1-D token tensors) -> the list of
+        prompts with ``max_new_tokens`` tokens each. The prompts are worked off packed, without padding, into a paged
+        cache; every further step is one token per request, by default replayed from a captured hipGraph on the GPU.
+        Prompt plus new tokens must fit the context. ``penalties`` as in ``generate``."""
+        was_training = self.training
+        self.eval()
+        try:
+            cfg, dev = self.config, self.lm_head.weight.device
+            prompts = [p.reshape(-1).to(device=dev, dtype=torch.int64) for p in prompts]
+            lens, R = [int(p.numel()) for p in prompts], len(prompts)
+            if R == 0 or min(lens) == 0 or max_new_tokens < 1:
+                raise ValueError("generate_ragged: at least one prompt, every prompt and max_new_tokens at least 1")
+            longest = max(lens) + max_new_tokens - 1       # the last token needs no row of the cache
+            pages = sum((n + max_new_tokens - 1 + page_size - 1) // page_size for n in lens)
+            cache = PagedKVCache(cfg, R, longest, pages, dev, self.lm_head.weight.dtype, page_size)
+            history = torch.zeros(R, max(lens) + max_new_tokens, dtype=torch.int64, device=dev)
+            for r, p in enumerate(prompts):
+                history[r, :lens[r]] = p
+            prompt_lens = torch.tensor(lens, dtype=torch.int32).to(dev)
+            total_lens = prompt_lens.clone()
+
+            def sample(logits):
+                if penalties:
+                    logits = ops.penalize_logits(logits[:, -1, :], history, prompt_lens, total_lens, **penalties)[:, None, :]
+                tok = self._sample(logits, temperature, topk, fused=True)
+                history.scatter_(1, total_lens[:, None].long(), tok)
+                total_lens.add_(1)
+                return tok
+
+            cache.begin(prompt_lens, sum(lens), max(lens))
+            logits, _, _ = self.forward(torch.cat(prompts)[None, :], kv_caches=cache)
+            cache.commit()
+            tok = sample(logits)                             # [R, 1]
+            one = torch.ones_like(prompt_lens)
+
+            def step():
+                cache.begin(one, R, 1)
+                lg, _, _ = self.forward(tok.view(1, R), kv_caches=cache)
+                cache.commit()
+                tok.copy_(sample(lg))
+
+            left = max_new_tokens - 1
+            self.last_decode_graphed = False
+            if (history.is_cuda if hip_graph is None else hip_graph and history.is_cuda) and left >= 2:
+                step()                                       # lazy initialisations happen outside the capture
+                graph = torch.cuda.CUDAGraph()
+                torch.cuda.synchronize()
+                with torch.cuda.graph(graph):
+                    step()
+                for _ in range(left - 1):
+                    graph.replay()
+                self.last_decode_graphed = True
+            else:
+                for _ in range(left):
+                    step()
+            return [history[r, :lens[r] + max_new_tokens].clone() for r in range(R)]
+        finally:
+            if was_training:
+                self.train()
