@@ -1546,6 +1546,7 @@ Tensor penalize_logits(const Tensor& logits, const std::optional<Tensor>& tokens
                     (o.stride(1) == 1 || V == 1),
                 who, ": out must look like the logits, with unit inner stride");
     at::assert_no_internal_overlap(o);
+    if (bias.has_value()) at::assert_no_overlap(o, *bias);
     at::assert_no_partial_overlap(o, logits);   // in place is fine: every element is read and written by one thread
   } else {
     o = at::empty({R, V}, logits.options());

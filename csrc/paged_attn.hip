@@ -9,7 +9,6 @@
 // lane = feature for the values, probabilities by broadcast; running maximum, sum and output in fp32.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "mfma_tiles.h"
 #include "paged.h"
@@ -1127,7 +1126,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kern
     if (!first_run) __syncthreads();                  // the last run's outputs have been read from LDS
     few_rows<T, W, RUN>(a, f, t, k0, k1, slot, smem, lds0, ml_s);
     if (!whole && s0 == 0 && tid == 0) {
-      const int last = (at + steps - 1) / per;        // the workgroup that has its end
+      const int last = min((at + steps - 1) / per, eff - 1);        // the workgroup that has its end
       write_meta(f, slot, last - id + 1, t.start, rows0, t.nrows, g, 2 * id, 2);
     }
     at += s1 - s0;
@@ -1274,7 +1273,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs
   const int* meta = f.meta + (long long)slot * 8;
   const int np = meta[0], start = meta[1], rows0 = meta[2], nrows = min(meta[3] - (int)blockIdx.y * kJoinRows, kJoinRows), g = meta[4];
   const int other = meta[5], stride = meta[6];
-  if (np < 2 || nrows <= 0) return;
+  if (np < 2 || nrows <= 0 || other + (np - 1) * stride >= f.max_slots) return;      // (lengths that contradict each other)
   const int row_b = blockIdx.y * kJoinRows, units = nrows * CPR;
   int groups = 1;
   while (2 * groups * units <= kThreads) groups *= 2;
@@ -1383,10 +1382,11 @@ template <typename T, int W, int RUN, bool CHUNKS>
 void launch_fast(const PagedAttnArgs& a, const FastArgs& f, int grid, hipStream_t st) {
   constexpr int lds = 4 * 2 * 32 * W * 2;
   auto kernel = CHUNKS ? paged_attn_kernel<T, W, RUN> : paged_attn_few_kernel<T, W, RUN>;
-  static bool set = false;       // above the default limit of dynamic LDS; the same value every time
-  if (!set) {
+  static bool set[64] = {};      // by device: above the default limit of dynamic LDS, the same value every time
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64 || !set[dev]) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    set = true;
+    if (dev >= 0 && dev < 64) set[dev] = true;
   }
   if (a.R > kWaveRequests) hipLaunchKernelGGL((paged_attn_items_kernel<CHUNKS>), dim3(1), dim3(1024), 0, st, a, f);
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, st, a, f);

@@ -89,7 +89,7 @@ def paged_plan(q_lens: torch.Tensor, ctx_lens: torch.Tensor, block_table: torch.
         kv.append(c + n)
     rest = num_tokens - cu[-1]
     had = min(taken, count)
-    return PagedPlan(*(torch.tensor(x, dtype=torch.int32) for x in
+    return PagedPlan(*(torch.tensor(x, dtype=torch.int32, device=q_lens.device) for x in
                        (cu, kv, positions + [0] * rest, slots + [-1] * rest, [count - had, wanted - had])))
 
 

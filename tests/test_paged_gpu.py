@@ -73,6 +73,14 @@ def test_plan_short_of_pages_columns_and_rows(count, cols, rows):
         assert torch.equal(a.cpu(), b), name
 
 
+def test_plan_without_requests_or_rows():
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    p = ops.paged_plan(none, none, torch.zeros(0, 3, dtype=torch.int32, device=DEV), none, i32(0), 16, 2)
+    assert p.cu_q.tolist() == [0] and p.slots.tolist() == [-1, -1] and p.positions.tolist() == [0, 0] and p.free_left.tolist() == [0, 0]
+    p = ops.paged_plan(i32(0, 0), i32(5, 0), torch.zeros(2, 1, dtype=torch.int32, device=DEV), i32(1), i32(1), 16, 0)
+    assert p.cu_q.tolist() == [0, 0, 0] and p.kv_lens.tolist() == [5, 0] and p.free_left.tolist() == [1, 0]
+
+
 # ---- append ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
 @pytest.mark.parametrize("N,nkv,dk,dv,page", [(1, 1, 64, 64, 16), (65, 12, 64, 64, 16), (300, 8, 128, 64, 24), (77, 3, 20, 7, 1), (130, 2, 96, 96, 5)])
@@ -119,16 +127,22 @@ def pool(kv, page, nkv, width, dtype, g, spare=2, columns=0):
 def bound(q, k, v, table, cu, kv, scale, window, n_max):
     """The exact result in 64 bits, and the error that the formula's roundings allow, element by element. With u the
     half step of the type: each probability may be rounded to the type before the product (u), the result is (u);
-    a score is an fp32 sum of width products (width + 4 roundings of its terms' size, at most |q| |k| scale) and moves
-    numerator and denominator; the sums over n keys are fp32. All relative to sum w |v|, which bounds |o|."""
+    a score is an fp32 sum of width products (width + 4 roundings of its terms' size, at most |q| |k| |scale|) and moves
+    numerator and denominator, whatever the scale's sign; the sums over n keys are fp32. All relative to sum w |v|, which bounds |o|."""
     exact = ops.paged_attention_eager(q.double(), k.double(), v.double(), table, cu, kv, scale, window)
     size = ops.paged_attention_eager(q.double(), k.double(), v.double().abs(), table, cu, kv, scale, window)
     u = half_step(q.dtype)
     kn = torch.nan_to_num(k.float(), 0.0, 0.0, 0.0).norm(dim=-1).max().item()
-    top = scale * q.float().norm(dim=-1).max().item() * kn
+    top = abs(scale) * q.float().norm(dim=-1).max().item() * kn
     f = 2.0 ** -24
     score = (q.shape[-1] + 4) * f * top + 4 * f * (1 + top)       # and the exponential with its argument
     return exact, size * (2 * u + 2 * score + (n_max + 4) * f) * 1.01 + torch.finfo(q.dtype).tiny
+
+
+def close(o, want, tol):
+    err = (o.double() - want).abs()
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert bool((err <= tol).all()), f"error up to {worst:.3f} of the bound"
 
 
 def check_attention(qn, ctx, nh, nkv, width, page, dtype, window=None, max_q=None, pad=0, gain=1.0):
@@ -143,9 +157,8 @@ def check_attention(qn, ctx, nh, nkv, width, page, dtype, window=None, max_q=Non
     cu, kv = i32(*cu), i32(*kv)
     o = ops.paged_attention(q, k, v, table, cu, kv, window=window, max_q=max_q)
     want, tol = bound(q, k, v, table, cu, kv, scale, window, max([1] + kv.tolist()))
-    err = (o.double() - want).abs()
     assert torch.isfinite(o).all()
-    assert (err <= tol).all(), f"worst {(err / tol).max().item():.3f} of the bound, at {(err - tol).argmax().item()}"
+    close(o, want, tol)
     return q, k, v, table, cu, kv, o
 
 
@@ -220,7 +233,7 @@ def test_attention_rising_and_falling_scores():
             cu, kv = i32(0, n), i32(600)
             o = ops.paged_attention(q[:n], k, v, table, cu, kv)
             want, tol = bound(q[:n], k, v, table, cu, kv, 1 / 8, None, 600)
-            assert ((o.double() - want).abs() <= tol).all()
+            close(o, want, tol)
 
 
 @pytest.mark.parametrize("n", [1, 3, 60, 200])
@@ -232,7 +245,7 @@ def test_attention_rows_before_the_first_key_are_zero(n):
     o = ops.paged_attention(q, k, v, table, cu, kv)
     assert (o[: n - n // 3] == 0).all() and (o[n:] == 0).all()
     want, tol = bound(q, k, v, table, cu, kv, 1 / 8, None, n)
-    assert ((o.double() - want).abs() <= tol).all()
+    close(o, want, tol)
 
 
 @pytest.mark.parametrize("n", [1, 100])
@@ -245,7 +258,7 @@ def test_attention_missing_pages_are_left_out(n, width):
     table[0, 0], table[0, 7], table[0, 24], table[1, 3] = -1, k.shape[0], 2 ** 31 - 1, -2 ** 31
     o = ops.paged_attention(q, k, v, table, cu, kv)
     want, tol = bound(q, k, v, table, cu, kv, 1 / math.sqrt(width), None, 400)
-    assert ((o.double() - want).abs() <= tol).all()
+    close(o, want, tol)
     table.fill_(-1)
     assert (ops.paged_attention(q, k, v, table, cu, kv) == 0).all()
 
@@ -272,12 +285,34 @@ def test_attention_values_in_masked_places_stay_there(n, window, width, bad):
     rest = [d for d in range(width) if d != 3]
     # elsewhere what the clean values give, within the formula's roundings: such tiles may be summed in another order
     want, tol = bound(q, k, torch.nan_to_num(v, 0.0, 0.0, 0.0), table, cu, kv, 1 / math.sqrt(width), window, L)
-    assert ((o[~sees].double() - want[~sees]).abs() <= tol[~sees]).all()
-    assert ((o[..., rest].double() - want[..., rest]).abs() <= tol[..., rest]).all()
+    close(o[~sees], want[~sees], tol[~sees])
+    close(o[..., rest], want[..., rest], tol[..., rest])
     v.view(-1, 2, width)[slot, :, 3] = 0
     k.view(-1, 2, width)[slot] = math.nan
     o = ops.paged_attention(q, k, v, table, cu, kv, window=window)
     assert torch.isfinite(o[~sees]).all() and torch.isnan(o[sees]).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, -3.0, 1e-8])
+@pytest.mark.parametrize("n", [2, 90])
+def test_attention_scales(scale, n):
+    """Zero: equal weights; negative: the order of the scores turned round."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    k, v, table = pool([200, 64], 16, 2, 64, BF, g)
+    q = torch.randn(2 * n, 4, 64, device=DEV, generator=g).to(BF)
+    cu, kv = i32(0, n, 2 * n), i32(200, 64)
+    for window in (None, 20):
+        o = ops.paged_attention(q, k, v, table, cu, kv, scale, window=window)
+        want, tol = bound(q, k, v, table, cu, kv, scale, window, 200)
+        close(o, want, tol)
+
+
+def test_attention_max_q_selects_kernels_not_results():
+    q, k, v, table, cu, kv, o = check_attention([1, 100, 3], [300, 50, 10], 8, 2, 64, 16, BF)
+    want, tol = bound(q, k, v, table, cu, kv, 1 / 8, None, 301)
+    for max_q in (1, 7, 100, 10 ** 9):
+        got = ops.paged_attention(q, k, v, table, cu, kv, max_q=max_q)
+        close(got, want, tol)
 
 
 def test_attention_strided_operands_and_out():
@@ -302,7 +337,7 @@ def test_attention_strided_operands_and_out():
     # rows that no 16-byte access can reach
     odd = torch.empty(k.numel() + 1, dtype=BF, device=DEV)[1:].view_as(k).copy_(k)
     want, tol = bound(q, k, v, table, cu, lens, 1 / 8, None, 200)
-    assert ((ops.paged_attention(q, odd, v, table, cu, lens).double() - want).abs() <= tol).all()
+    close(ops.paged_attention(q, odd, v, table, cu, lens), want, tol)
 
 
 def test_attention_leaves_rows_outside_the_requests():
@@ -439,7 +474,7 @@ def test_steps_of_a_ragged_batch_match_one_pass():
     for r, n in enumerate(lens):
         mine = i32(0).view(1, 1)
         want, tol = bound(qs[r], ks[r][None], vs[r][None], mine, i32(0, n), i32(n), 1 / 8, None, n)
-        assert ((torch.cat(outs[r]).double() - want).abs() <= tol).all()
+        close(torch.cat(outs[r]), want, tol)
 
 
 def test_captured_steps_follow_their_buffers():
@@ -568,6 +603,7 @@ def test_refusals_on_the_gpu():
         lambda: ops.penalize_logits(lg, torch.zeros(2, 3, device=DEV)), lambda: ops.penalize_logits(lg, bias=lg[:, :3]),
         lambda: ops.penalize_logits(lg, bias=lg.half()), lambda: ops.penalize_logits(lg, allowed=i32(0)),
         lambda: ops.penalize_logits(lg, out=lg[:, :39]), lambda: ops.penalize_logits(lg.double()),
+        lambda: ops.penalize_logits(lg, bias=lg, out=lg),
         lambda: ops.penalize_logits(lg, total_lens=i32(1, 2, 3)), lambda: ops.penalize_logits(lg, repetition=torch.ones(2)),
     ]
     for i, call in enumerate(bad):
