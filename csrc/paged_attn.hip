@@ -115,9 +115,23 @@ __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAt
 // sum per lane, O^T += V^T P^T with V read transposed from LDS.
 //
 // Lengths live on the device, so every workgroup derives the list of items from them (one pass over the requests:
-// R <= 256 is one load per thread) and takes the one of its number. The keys of a request are cut into pieces when
-// there are fewer items than `target`; the pieces leave (O, reference, sum) in the workspace and a second kernel joins
-// them, in the order of the keys, so a result does not depend on which workgroup ran when.
+// R <= 256 is one load per lane or thread; more go through one more kernel). Few rows alone (paged_attn_few_kernel) take
+// equal shares of all 128-key steps, one round of workgroups whatever the lengths. Chunks (paged_attn_kernel, few rows
+// among them) take items; their keys are cut into pieces when there are fewer items than `target`. What is cut leaves
+// (O, reference, sum) in the workspace and a second kernel joins it, in the order of the keys: a result does not
+// depend on which workgroup ran when. The second kernel costs 4 - 6 us of every call.
+//
+// Measured (large copy on the same card 4.9 TB/s, plain reads 6.2, a large bf16 product 1.48 PF/s):
+//   64 requests x 2000-8000 keys, 32 / 8 heads of 128, bf16      213 us   5.9 TB/s: the bytes
+//   2 requests x 33 K-131 K keys, same heads, fp16               105 us   5.8 TB/s
+//   8 requests x 250-1000 keys, 12 heads of 64, bf16              17 us   four dependent trips to memory (lengths, table,
+//                                                                         keys, join) on a quarter-empty card
+//   8 prompts of 1000-3000 rows on 500-2000 cached, 32 / 8 x 128  655 us  0.84 PF/s: the LDS pipe (transposed reads) and
+//                                                                         the vector instructions of the softmax
+//
+// Two things the loops live from, both found in the compiler's waits: nothing in them may spill (a reload is a
+// vector-memory wait, which waits for the transfers in flight: 737 -> 1232 us on the prompts), so what is rare is done
+// elsewhere (exact_rows); and no register that an ordinary load fills may have its first use in them (load_row).
 //
 // The score's reference point mb (log2 units) moves only when a subtile's maximum passes it by 2^8: p <= 2^(kBias + 8).
 // kBias = 6 for fp16 keeps small probabilities out of its subnormal range (one of 2^-20 still has all its bits).
@@ -331,7 +345,7 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
 // A (request, 32 packed rows, KV head) is a run of 128-key steps (one at least); the runs lie one after another, and workgroup i of `eff`
 // takes steps [i * per, (i + 1) * per) of them all, whichever runs they fall into: contexts of any mix of lengths load
 // the card evenly in one round. At most its first and its last run are cut.
-constexpr int kMinSteps = 1;           // fewer steps than this are not worth a workgroup of their own
+constexpr int kMinSteps = 1;           // steps worth a workgroup of their own (8 x 1k keys: 17.2 us; 2: 19.7, 4: 20.9, 8, uncut: 31.7)
 __device__ __forceinline__ int run_base(const Request& q) { return q.klo & ~31; }
 __device__ __forceinline__ int run_steps(const Request& q) {
   return q.rows > 0 ? max((q.khi - run_base(q) + kFewStep - 1) / kFewStep, 1) : 0;
@@ -1358,7 +1372,7 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
   p.chunks = (long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows;
   if (p.chunks) {
-    p.target = num_cus * 2;
+    p.target = num_cus * 2;         // (4: 43 instead of 37 us on a mixed batch of 33 requests, no difference on prompts)
     // tiles: one per request with rows, and one more for every 128 rows of a chunk
     const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
     p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);

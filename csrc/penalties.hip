@@ -9,7 +9,9 @@
 // LDS atomics: the result does not depend on their order. Bound by the logits' bytes at serving batches and by
 // latency at a few rows, so the slice is what fills the card: a whole row's worth of it costs one pass over the
 // history per slice, a short one spreads a few rows over many CUs. Counters have 16 bits while the history cannot
-// overflow the 15 of the count.
+// overflow the 15 of the count. Measured: one row of 50304 bf16 4.0 us (7.3 us a call from Python); 256 rows fp32 with
+// bias, mask and 2000-4000 tokens of history 33 us, 5.0 TB/s (8192 entries to a slice with 32-bit counters and single
+// elements: 69 us).
 #include <algorithm>
 
 #include "paged.h"
