@@ -1373,8 +1373,12 @@ void paged_append(Tensor k_pages, Tensor v_pages, const Tensor& k, const Tensor&
   at::assert_no_internal_overlap(k_pages);
   at::assert_no_internal_overlap(v_pages);
   at::assert_no_overlap(k_pages, v_pages);
+  for (const Tensor* t : {&k, &v}) {
+    at::assert_no_overlap(k_pages, *t);
+    at::assert_no_overlap(v_pages, *t);
+  }
   check_int_vec(slots, k.size(0), k_pages, who, "slots");
-  TORCH_CHECK(k.size(0) < (1 << 30) && page <= (1 << 20) && H * (k.size(2) + v.size(2)) < (1 << 20), who, ": size out of range");
+  TORCH_CHECK(k.size(0) < (1 << 24) && page <= (1 << 20) && H * (k.size(2) + v.size(2)) < (1 << 20), who, ": size out of range");
   c10::DeviceGuard guard(k_pages.device());
   dpa::PagedAppendArgs a{};
   a.k_pages = k_pages.data_ptr();
@@ -1428,7 +1432,10 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
               who, ": block_table must be int32 [requests, columns] with unit inner stride on the same device");
   TORCH_CHECK(table.size(1) * k_pages.size(1) < (int64_t(1) << 30) && k_pages.size(1) <= (1 << 20), who,
               ": more than 2^30 rows per request");
-  TORCH_CHECK(N < (1 << 29) && R < (1 << 29) && N * nh < (int64_t(1) << 31), who, ": too many rows");
+  // (the last: workgroups of 256 threads, fewer than 2^32 in all)
+  TORCH_CHECK(N < (1 << 29) && R < (1 << 29) && N * nh < (int64_t(1) << 31) &&
+                  std::min(N, R) * nkv + N * nh / 128 < (int64_t(15) << 20),
+              who, ": too many rows");
   TORCH_CHECK(window >= 0 && window < (int64_t(1) << 31), who, ": window must be positive (0: none)");
   TORCH_CHECK(max_q >= 0, who, ": max_q must not be negative");
   TORCH_CHECK(std::isfinite(scale), who, ": scale must be finite");
@@ -1440,7 +1447,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
                     (o.stride(2) == 1 || W == 1),
                 who, ": out must look like q, with unit inner stride");
     at::assert_no_internal_overlap(o);
-    at::assert_no_overlap(o, q);
+    for (const Tensor* t : {&q, &k_pages, &v_pages}) at::assert_no_overlap(o, *t);
   } else {
     o = at::empty({N, nh, W}, q.options());
   }
@@ -1473,7 +1480,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.page = (int)k_pages.size(1);
   a.by_page = dpa::make_fast_div(a.page);
   a.scale = (float)scale;
-  a.window = (int)window;
+  a.window = window < (1 << 30) ? (int)window : 0;   // positions are below 2^30: a wider one hides nothing
   a.max_q = (int)std::min<int64_t>(max_q > 0 ? max_q : N, N);
   a.type = type;
   a.zero_rest = !out.has_value();

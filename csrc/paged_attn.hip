@@ -35,7 +35,7 @@ template <typename T>
 __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAttnArgs a) {
   __shared__ float q_s[kGenWaves][kGenWidth];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long id = (long long)blockIdx.x * kGenWaves + wave;
+  const long long id = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kGenWaves + wave;
   if (id >= (long long)a.N * a.nh) return;     // whole waves; no workgroup barrier below
   const int i = (int)(id / a.nh), h = (int)(id % a.nh), g = h / (a.nh / a.nkv);
   T* o = (T*)a.o + (long long)i * a.o_ts + (long long)h * a.o_hs;
@@ -1370,7 +1370,9 @@ struct Plan {
 Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   Plan p;
   const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
-  p.chunks = (long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows;
+  // (the 128-key steps of all runs are counted in 32 bits; pages shared by many long requests could pass that)
+  const long long steps = (a.R + (long long)a.N * G / kFewRows) * a.nkv * ((long long)a.M * a.page / kFewStep + 2);
+  p.chunks = ((long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows) || steps >= (1ll << 31);
   if (p.chunks) {
     p.target = num_cus * 2;         // (4: 43 instead of 37 us on a mixed batch of 33 requests, no difference on prompts)
     // tiles: one per request with rows, and one more for every 128 rows of a chunk
@@ -1453,7 +1455,8 @@ void paged_attn(const PagedAttnArgs& a, int num_cus, void* workspace, hipStream_
     return;
   }
   const long long waves = (long long)a.N * a.nh;
-  const dim3 grid((unsigned)((waves + kGenWaves - 1) / kGenWaves)), block(kGenWaves * 64);
+  const long long groups = (waves + kGenWaves - 1) / kGenWaves, gx = std::min(groups, 1ll << 20);
+  const dim3 grid((unsigned)gx, (unsigned)((groups + gx - 1) / gx)), block(kGenWaves * 64);
   if (a.type == kTypeBf16) hipLaunchKernelGGL((paged_attn_rows_kernel<bf16_t>), grid, block, 0, st, a);
   else if (a.type == kTypeHalf) hipLaunchKernelGGL((paged_attn_rows_kernel<half_t>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((paged_attn_rows_kernel<float>), grid, block, 0, st, a);

@@ -97,7 +97,8 @@ def paged_plan(q_lens: torch.Tensor, ctx_lens: torch.Tensor, block_table: torch.
 def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Rows ``k, v [N, nkv, width]`` (any strides with unit inner stride, e.g. the columns of a fused projection) into
     rows ``slots [N]`` of the pools ``[P, page, nkv, width]`` (any page, row and head strides). Slots outside
-    ``[0, P * page)`` are skipped; the others must be distinct. Key and value widths may differ."""
+    ``[0, P * page)`` are skipped; the others must be distinct. Key and value widths may differ; the new rows lie outside
+    the pools."""
     if use_hip(k_pages, k):
         ops().paged_append(k_pages, v_pages, k, v, slots)
         return

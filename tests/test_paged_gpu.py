@@ -246,6 +246,24 @@ def test_attention_rows_before_the_first_key_are_zero(n):
     assert (o[: n - n // 3] == 0).all() and (o[n:] == 0).all()
     want, tol = bound(q, k, v, table, cu, kv, 1 / 8, None, n)
     close(o, want, tol)
+    # a window past every position hides nothing (and does not pass 32 bits at rows of negative position)
+    for window in (2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1):
+        assert torch.equal(ops.paged_attention(q, k, v, table, cu, kv, window=window), o)
+        f = ops.paged_attention(q.float(), k.float(), v.float(), table, cu, kv, window=window)
+        assert (f[: n - n // 3] == 0).all() and (f[n:] == 0).all()
+
+
+def test_attention_of_more_steps_than_32_bits_count():
+    """512 requests whose tables could name 2^29 rows each: the capacity, not the lengths, decides the kernel."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    R, page = 512, 1 << 20
+    k = torch.randn(1, page, 1, 64, device=DEV, generator=g).to(BF)
+    v = torch.randn(1, page, 1, 64, device=DEV, generator=g).to(BF)
+    table = torch.zeros(R, 512, dtype=torch.int32, device=DEV)
+    q = torch.randn(R, 2, 64, device=DEV, generator=g).to(BF)
+    cu, kv = torch.arange(R + 1, dtype=torch.int32, device=DEV), i32(*[(37 * r) % 900 + 1 for r in range(R)])
+    want, tol = bound(q, k, v, table, cu, kv, 1 / 8, None, 900)
+    close(ops.paged_attention(q, k, v, table, cu, kv, max_q=1), want, tol)
 
 
 @pytest.mark.parametrize("n", [1, 100])
@@ -583,6 +601,7 @@ def test_refusals_on_the_gpu():
     v = k.clone()
     row = torch.zeros(1, 1, 8, device=DEV)
     lg = torch.zeros(2, 40, device=DEV)
+    many = torch.zeros(1 << 24, dtype=torch.int32, device=DEV)
     bad = [
         lambda: ops.paged_plan(one.long(), one, t, one, one, 4, 1), lambda: ops.paged_plan(one, i32(1, 2), t, one, one, 4, 1),
         lambda: ops.paged_plan(one, one, t, one, one, 0, 1), lambda: ops.paged_plan(one, one, t, one, one, 4, -1),
@@ -592,6 +611,11 @@ def test_refusals_on_the_gpu():
         lambda: ops.paged_append(k, v, row, row, i32(1, 2)), lambda: ops.paged_append(k, k, row, row, one),
         lambda: ops.paged_append(k, v, row, row, one.cpu()), lambda: ops.paged_append(k.double(), v.double(), row.double(), row.double(), one),
         lambda: ops.paged_append(k[:, :1].expand(2, 4, 1, 8), v, row, row, one),
+        lambda: ops.paged_append(k, v, k.view(-1, 1, 8)[:1], row, one), lambda: ops.paged_append(k, v, row, k.view(-1, 1, 8)[:1], one),
+        lambda: ops.paged_append(k, v, row.expand(1 << 24, 1, 8), row.expand(1 << 24, 1, 8), many),
+        lambda: ops.paged_attention(row.expand(1 << 24, 1, 8), k, v, t.expand(1 << 24, 2), torch.cat([many, one]), many),
+        lambda: ops.paged_attention(q, k, v, t, cu, one, out=k.view(4, 2, 8)[:1]),
+        lambda: ops.paged_attention(q, k, v, t, cu, one, out=v.view(4, 2, 8)[:1]),
         lambda: ops.paged_attention(q[..., :4], k, v, t, cu, one), lambda: ops.paged_attention(q, k, v, t, cu, i32(1, 1)),
         lambda: ops.paged_attention(q, k, v, t.long(), cu, one), lambda: ops.paged_attention(q, k, v, t, cu, one, window=0),
         lambda: ops.paged_attention(q, k, v, t, cu, one, out=q), lambda: ops.paged_attention(q.half(), k, v, t, cu, one),
