@@ -1091,20 +1091,22 @@ class LLM(nn.Module):
                 cache.commit()
                 tok.copy_(sample(lg))
 
-            left = max_new_tokens - 1
-            self.last_decode_graphed = False
+            left, graph = max_new_tokens - 1, None
             if (history.is_cuda if hip_graph is None else hip_graph and history.is_cuda) and left >= 2:
                 step()                                       # lazy initialisations happen outside the capture
+                left -= 1
                 graph = torch.cuda.CUDAGraph()
                 torch.cuda.synchronize()
-                with torch.cuda.graph(graph):
-                    step()
-                for _ in range(left - 1):
-                    graph.replay()
-                self.last_decode_graphed = True
-            else:
-                for _ in range(left):
-                    step()
+                try:
+                    with torch.cuda.graph(graph):
+                        step()
+                except Exception as exc:                     # some op of this configuration cannot be captured
+                    torch.cuda.synchronize()
+                    print(f"[hip_graph] decode capture failed ({type(exc).__name__}: {exc}); decoding eagerly", flush=True)
+                    graph = None
+            self.last_decode_graphed = graph is not None
+            for _ in range(left):
+                step() if graph is None else graph.replay()
             return [history[r, :lens[r] + max_new_tokens].clone() for r in range(R)]
         finally:
             if was_training:

@@ -148,6 +148,24 @@ def test_ragged_generation_on_the_gpu(penalties):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("capture", [True, False])
+def test_ragged_generation_with_experts(capture, monkeypatch):
+    """Whether or not the step can be captured, the tokens are those of the eager steps."""
+    m = model_of("mqa_sin_moe", BIG, "cuda", torch.bfloat16)
+    prompts = [torch.randint(0, 512, (n,), device="cuda") for n in (70, 2, 33)]
+    eager = m.generate_ragged(prompts, 12, topk=1, hip_graph=False)
+    assert not m.last_decode_graphed
+    if not capture:
+        def refuse(*a, **k):
+            raise RuntimeError("not captured")
+        monkeypatch.setattr(torch.cuda, "graph", refuse)
+    out = m.generate_ragged(prompts, 12, topk=1)
+    assert capture or not m.last_decode_graphed
+    for a, b in zip(eager, out):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_penalties_in_the_captured_dense_step():
     m = model_of("mha_learn", BIG, "cuda", torch.bfloat16)
     idx = torch.randint(0, 512, (3, 9), device="cuda")
