@@ -724,62 +724,58 @@ __device__ __forceinline__ bool subtile(const char* kt, const char* vt, int ks0,
   return rare;
 }
 
-// NS 32-key subtiles of a chunk's tile, from key ks0 on. No maximum is taken as a rule: the probabilities come from the
+// A 32-key subtile of a chunk, from key ks0 on. No maximum is taken as a rule: the probabilities come from the
 // reference as it is, and what they sum to says whether it still serves (fp32 sums and the 16-bit operand keep their
 // relative precision whatever the magnitude; kSumMax keeps fp16 finite). If it does not, or a row has none yet, the
-// scores are computed again and the reference moves to their maximum.
-template <typename T, int W, int NS>
+// scores are computed again and the reference moves to their maximum. (Two subtiles taken together: 668 instead of 653
+// us on the 16k prompts, fewer registers to schedule with.)
+// Behind the score products a wave goes before the others of its SIMD: one is then in its softmax and value products
+// while another waits for its keys, where equals would do both at the same time (16k prompts 665 -> 640 us, mixed batch
+// 35.2 -> 33.7; from the key reads on 648, for the products alone 664, for the softmax alone 664).
+template <typename T, int W>
 __device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int ks0, bool mask, float c, const u32x4 (&qf)[W / 16],
                                            RowState<W>& st, int lane) {
   typedef Frag<T> F;
-  constexpr int NK = W / 16, ND = W / 32, SUB = 32 * W * 2;
+  constexpr int NK = W / 16, ND = W / 32;
   constexpr float kSumMax = F::kBias ? 32768.f : 1.0e9f;
   const int r = lane & 31, hh = lane >> 5;
-  f32x16 s[NS];
+  f32x16 s;
   auto scores = [&]() {
+    u32x4 kf[NK];
 #pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      u32x4 kf[NK];
+    for (int ks = 0; ks < NK; ++ks) kf[ks] = __builtin_bit_cast(u32x4, row_frag<W>(kt, r, ks, hh));
+    __builtin_amdgcn_sched_barrier(0);     // all fragments requested before the first product
 #pragma unroll
-      for (int ks = 0; ks < NK; ++ks) kf[ks] = __builtin_bit_cast(u32x4, row_frag<W>(kt + h * SUB, r, ks, hh));
-      __builtin_amdgcn_sched_barrier(0);     // all fragments requested before the first product
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < NK; ++ks) s[h] = F::mfma(kf[ks], qf[ks], s[h]);
-    }
+    for (int ks = 0; ks < NK; ++ks) s = F::mfma(kf[ks], qf[ks], s);
+    __builtin_amdgcn_s_setprio(1);
     if (mask) {
       const int lo_rel = st.lo - ks0 - 4 * hh, hi_rel = st.hi - ks0 - 4 * hh;
 #pragma unroll
-      for (int h = 0; h < NS; ++h)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = 32 * h + acc_row(i, 0);
-          if (key < lo_rel || key > hi_rel) s[h][i] = -INFINITY;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int key = acc_row(i, 0);
+        if (key < lo_rel || key > hi_rel) s[i] = -INFINITY;
+      }
     }
   };
   auto weights = [&]() {
     const float base = st.mb == -INFINITY ? 0.f : st.mb;      // a row that sees nothing yet: every s is -inf
     float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int h = 0; h < NS; ++h)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], c, -base));
-        sum[i & 1] += s[h][i];
-      }
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));
+      sum[i & 1] += s[i];
+    }
     return sum[0] + sum[1];
   };
   scores();
   float rs = weights();
   if (!__all(rs <= kSumMax && (st.mb != -INFINITY || st.hi < 0))) {
     scores();
-    float mx = s[0][0];
+    float mx = s[0];
 #pragma unroll
-    for (int h = 0; h < NS; ++h)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
     const float to = max_halves(mx) * c - (float)F::kBias;
     const bool move = to > st.mb;
     const float alpha = move ? __builtin_amdgcn_exp2f(st.mb - to) : 1.f;
@@ -792,25 +788,23 @@ __device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int k
     rs = weights();
   }
   st.l += rs;
+  u32x4 vf[2][ND];
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) vf[s2][dt] = __builtin_bit_cast(u32x4, tr_frag<W>(vt, 0, s2, dt, lane));
+  __builtin_amdgcn_sched_barrier(0);
   bool rare = false;
+  if (mask) rare = not_finite<T, W>(vf);
 #pragma unroll
-  for (int h = 0; h < NS; ++h) {
-    u32x4 vf[2][ND];
+  for (int s2 = 0; s2 < 2; ++s2) {
+    u32x4 pb;
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
+    for (int j = 0; j < 4; ++j) pb[j] = F::pack(s[8 * s2 + 2 * j], s[8 * s2 + 2 * j + 1]);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) vf[s2][dt] = __builtin_bit_cast(u32x4, tr_frag<W>(vt + h * SUB, 0, s2, dt, lane));
-    __builtin_amdgcn_sched_barrier(0);
-    if (mask) rare |= not_finite<T, W>(vf);
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      u32x4 pb;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) pb[j] = F::pack(s[h][8 * s2 + 2 * j], s[h][8 * s2 + 2 * j + 1]);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) st.o[dt] = F::mfma(vf[s2][dt], pb, st.o[dt]);
-    }
+    for (int dt = 0; dt < ND; ++dt) st.o[dt] = F::mfma(vf[s2][dt], pb, st.o[dt]);
   }
+  __builtin_amdgcn_s_setprio(0);
   return rare;
 }
 
@@ -1153,7 +1147,6 @@ template <typename T, int W, int RUN>
 __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArgs& f, const Tile& t, int k0, int k1,
                                            char* smem, unsigned lds0, int wave, int lane, u32x4 (&qf)[W / 16], RowState<W>& st) {
   constexpr int SUB = 32 * W * 2, NP = 2 * SUB / 1024 / 4, STAGE = 4 * SUB;   // transfers per wave and tile; a K and a V tile
-  constexpr int NS = 1;       // subtiles taken together; 2: 668 instead of 653 us on the 16k prefill (fewer registers to schedule with)
   const int r32 = lane & 31, hh = lane >> 5;
   PageRows<W, NP, RUN> pr;
   pr.init(a, t.table, t.g, t.klo, t.khi, lane);
@@ -1187,20 +1180,21 @@ __device__ __forceinline__ bool chunk_loop(const PagedAttnArgs& a, const FastArg
     stage ^= 1;
     if (!wave_live) continue;
 #pragma unroll 1
-    for (int ks0 = kt0; ks0 < kt0 + 64; ks0 += 32 * NS) {
+    for (int ks0 = kt0; ks0 < kt0 + 64; ks0 += 32) {
       if (ks0 > wp_last || ks0 >= t.khi) break;
-      if (a.window > 0 && ks0 + 32 * NS - 1 < wp_first - a.window + 1) continue;
-      const bool mask = ks0 + 32 * NS - 1 > wp_first || ks0 + 32 * NS > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
+      if (a.window > 0 && ks0 + 31 < wp_first - a.window + 1) continue;
+      const bool mask = ks0 + 31 > wp_first || ks0 + 32 > t.cap || (a.window > 0 && ks0 < wp_last - a.window + 1);
       const int at = (ks0 - kt0) * W * 2;
-      rare |= chunk_tile<T, W, NS>(kt + at, vt + at, ks0, mask, f.c, qf, st, lane);
+      rare |= chunk_tile<T, W>(kt + at, vt + at, ks0, mask, f.c, qf, st, lane);
     }
   }
   return rare;
 }
 
-// Chunks, with few-row requests among them.
+// Chunks, with few-row requests among them. Four workgroups on a CU at width 64 (8 x 2048 rows of 16 heads 124 -> 121 us;
+// two: 157), unless lanes hold addresses of their own (RUN 0), which takes the registers.
 template <typename T, int W, int RUN>
-__global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
+__global__ __launch_bounds__(kThreads, W == 64 ? (RUN > 0 ? 4 : 3) : 2) void paged_attn_kernel(PagedAttnArgs a, FastArgs f) {
   constexpr int ND = W / 32, SUB = 32 * W * 2, REGION = 2 * SUB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float ml_s[4][32][2];
