@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAt
 //   2 requests x 33 K-131 K keys, same heads, fp16               105 us   5.8 TB/s
 //   8 requests x 250-1000 keys, 12 heads of 64, bf16              17 us   four dependent trips to memory (lengths, table,
 //                                                                         keys, join) on a quarter-empty card
-//   8 prompts of 1000-3000 rows on 500-2000 cached, 32 / 8 x 128  655 us  0.84 PF/s: the LDS pipe (transposed reads) and
+//   8 prompts of 1000-3000 rows on 500-2000 cached, 32 / 8 x 128  640 us  0.86 PF/s: the LDS pipe (transposed reads) and
 //                                                                         the vector instructions of the softmax
 //
 // Two things the loops live from, both found in the compiler's waits: nothing in them may spill (a reload is a
@@ -180,7 +180,7 @@ struct FastArgs {
   float* ml;           // [max_slots][slot_rows][2] reference, sum
   int* meta;           // [max_slots][8]
   int* header;         // [0] = slots in use, [1], [2] = keys per piece
-  int* prefix;         // R > kWaveRequests: [2][R + 1] items and slots before each request
+  int* prefix;         // R > kWaveRequests: [3][R + 1] first items (few rows: steps), slots and second items before each request
 };
 
 // 256 zero bytes: what rows that no query may see, and pages that do not exist, read as
@@ -274,7 +274,10 @@ __device__ __forceinline__ int find_prefix(const int* prefix, int R, int x, int 
 struct Item {
   int r, j, slot, np;      // request, number inside it, slot of its output, pieces of its keys; r < 0: none
 };
-// Item `id`, found by one wave; every wave of the grid comes to the same list.
+// Item `id`, found by one wave; every wave of the grid comes to the same list. The list goes over the requests twice,
+// first the last two thirds of each one's tiles, which see most, then the others: the card runs out of work on short
+// items while those that run together still share a request's keys (8 x 2048 rows of 16 heads of 64 123 -> 112 us, mixed
+// batch 36.5 -> 35.4, no difference on the 16k prompts; halves 115 us, three quarters 119).
 __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs& f, int id, int lane) {
   Item it;
   it.r = -1;
@@ -292,20 +295,32 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
       }
     }
     const PieceSize size = piece_size(wave_total(cost), a.nkv, f.target);
-    int items[PER], slots[PER], ni = 0, ns = 0;
+    int items[PER], ahead[PER], slots[PER], n1 = 0, n2 = 0, ns = 0;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      items[u] = slots[u] = 0;
+      items[u] = ahead[u] = slots[u] = 0;
       if (q[u].tiles > 0) {
         const int np = pieces(q[u], size);
-        items[u] = q[u].tiles * np * a.nkv;
-        slots[u] = np > 1 ? items[u] : 0;
+        ahead[u] = (q[u].tiles - q[u].tiles / 3) * np * a.nkv;
+        items[u] = q[u].tiles / 3 * np * a.nkv;
+        slots[u] = np > 1 ? ahead[u] + items[u] : 0;
       }
-      ni += items[u];
+      n1 += ahead[u];
+      n2 += items[u];
       ns += slots[u];
     }
-    const int pi = wave_scan(ni), ps = wave_scan(ns);
+    const int p1 = wave_scan(n1), p2 = wave_scan(n2), ps = wave_scan(ns);
     if (id == 0 && lane == 63) f.header[0] = min(ps, f.max_slots);
+    const int all1 = __builtin_amdgcn_readlane(p1, 63);
+    const bool second = id >= all1;
+    const int pi = second ? p2 : p1, ni = second ? n2 : n1;
+    id -= second ? all1 : 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+      if (!second) {
+        items[u] = ahead[u];
+        ahead[u] = 0;
+      }
     const unsigned long long here = __ballot(id >= pi - ni && id < pi);
     if (here == 0ull) return it;
     const int src = __builtin_ctzll(here);
@@ -321,17 +336,22 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
     int np = 1;
 #pragma unroll
     for (int v = 0; v < PER; ++v)
-      if (u == v && q[v].tiles > 0) np = pieces(q[v], size);
+      if (u == v && q[v].tiles > 0) {
+        np = pieces(q[v], size);
+        first -= ahead[v];
+      }
     it.r = src * ((a.R + 63) >> 6) + __builtin_amdgcn_readlane(u, src);
     it.j = id - __builtin_amdgcn_readlane(first, src);
     it.slot = __builtin_amdgcn_readlane(slot, src) + it.j;
     it.np = __builtin_amdgcn_readlane(np, src);
     return it;
   }
-  const int lo = find_prefix(f.prefix, a.R, id, lane);
+  const int* const second = f.prefix + 2 * (a.R + 1);
+  const int all1 = f.prefix[a.R];
+  const int lo = id < all1 ? find_prefix(f.prefix, a.R, id, lane) : find_prefix(second, a.R, id - all1, lane);
   if (lo < 0) return it;
   it.r = lo;
-  it.j = id - f.prefix[lo];
+  it.j = id < all1 ? id - f.prefix[lo] : f.prefix[lo + 1] - f.prefix[lo] + id - all1 - second[lo];
   it.slot = f.prefix[a.R + 1 + lo] + it.j;
   const Request q = request(a, f, lo);
   PieceSize size;
@@ -410,7 +430,7 @@ __device__ __forceinline__ int find_run(const PagedAttnArgs& a, const FastArgs& 
 template <bool CHUNKS>
 __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a, FastArgs f) {
   __shared__ float red_f[16];
-  __shared__ int red_i[16], red_s[16];
+  __shared__ int red_i[16], red_s[16], red_2[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float cost = 0.f;
   if (CHUNKS) {
@@ -418,41 +438,48 @@ __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a,
     cost = block_sum(cost, red_f);
   }
   const PieceSize size = piece_size(cost, a.nkv, f.target);
-  int base_i = 0, base_s = 0;
+  int base_i = 0, base_s = 0, base_2 = 0;
   for (int r0 = 0; r0 < a.R; r0 += 1024) {
     const int r = r0 + tid;
-    int ni = 0, ns = 0;
+    int ni = 0, ns = 0, n2 = 0;
     if (r < a.R) {
       const Request q = request(a, f, r);
       const int np = CHUNKS ? pieces(q, size) : 1;
-      ni = CHUNKS ? q.tiles * np * a.nkv : run_steps(q) * run_count(q, a.nkv);
-      ns = np > 1 ? ni : 0;
+      ni = CHUNKS ? (q.tiles - q.tiles / 3) * np * a.nkv : run_steps(q) * run_count(q, a.nkv);
+      n2 = CHUNKS ? q.tiles / 3 * np * a.nkv : 0;
+      ns = np > 1 ? ni + n2 : 0;
     }
-    int pi = wave_scan(ni), ps = wave_scan(ns);
+    int pi = wave_scan(ni), ps = wave_scan(ns), p2 = wave_scan(n2);
     if (lane == 63) {
       red_i[wave] = pi;
       red_s[wave] = ps;
+      red_2[wave] = p2;
     }
     __syncthreads();
-    int ti = 0, ts = 0;
+    int ti = 0, ts = 0, t2 = 0;
     for (int w = 0; w < 16; ++w) {
       if (w == wave) {
         pi += ti;
         ps += ts;
+        p2 += t2;
       }
       ti += red_i[w];
       ts += red_s[w];
+      t2 += red_2[w];
     }
     if (r < a.R) {
       f.prefix[r] = base_i + pi - ni;
       f.prefix[a.R + 1 + r] = base_s + ps - ns;
+      f.prefix[2 * (a.R + 1) + r] = base_2 + p2 - n2;
     }
     base_i += ti;
     base_s += ts;
+    base_2 += t2;
     __syncthreads();
   }
   if (tid == 0) {
     f.prefix[a.R] = base_i;
+    f.prefix[3 * a.R + 2] = base_2;
     if (CHUNKS) f.header[0] = min(base_s, f.max_slots);
     f.header[1] = size.few;
     f.header[2] = size.chunk;
@@ -1384,7 +1411,7 @@ Plan plan_items(const PagedAttnArgs& a, int num_cus) {
   p.part = up((size_t)p.slots * p.slot_rows * W * 4);
   p.ml = up((size_t)p.slots * p.slot_rows * 8);
   p.meta = up((size_t)p.slots * 32);
-  p.total = p.part + p.ml + p.meta + 256 + (a.R > kWaveRequests ? up((size_t)(a.R + 1) * 8) : 0);
+  p.total = p.part + p.ml + p.meta + 256 + (a.R > kWaveRequests ? up((size_t)(a.R + 1) * 12) : 0);
   return p;
 }
 
