@@ -11,6 +11,9 @@
 //      walk of the one thread's registers in which u * total falls (u uniform in [0, 1) from a hash of the
 //      seed and the row). The order of the walk is a fixed permutation of the vocabulary, which a
 //      multinomial draw does not care about.
+// Logits of -inf (masked tokens) are never kept, whatever top-k says: the fp32 scan leaves a few of the 2^24 draws
+// outside every thread's interval, and those end on a token of positive weight too. A row of nothing but -inf gives
+// token 0; logits of +inf share the draw equally. A row with a NaN gives some token of the vocabulary.
 // Decode-step form (SampleStep): the kernel also records the token in the generation's history at the device-side
 // column, and the last workgroup to finish advances the step's device counters (cache position, fill level,
 // history column), so a captured decode step needs no bookkeeping launches and no per-step seed draw.
@@ -33,7 +36,8 @@ __device__ __forceinline__ unsigned smix32(unsigned x) {
   return x;
 }
 
-// Monotone map float -> uint32 (larger float, larger key). NaN sorts above +inf; callers feed finite logits.
+// Monotone map float -> uint32 (larger float, larger key). NaN sorts above +inf or below -inf, by its sign.
+constexpr unsigned kLowestKey = 0x00800000u;   // of the lowest finite float; that of -inf is one less
 __device__ __forceinline__ unsigned order_key(float x) {
   const unsigned b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_topk_kernel(const T* __
   const float tmax = mx;   // this thread's own maximum
   mx = block_max(mx, red);
 
-  unsigned thr_key = 0u;   // keep everything
+  unsigned thr_key = kLowestKey;   // keep everything but -inf
   bool found = false;
   constexpr int kLow = sizeof(T) == 2 ? 16 : 0;   // bf16 images have no low 16 bits
   if (topk > 0 && topk < V && topk <= kSampleThreads / 2) {
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_topk_kernel(const T* __
       if (lane == 0) found_key = bnd;
     }
     __syncthreads();
-    const unsigned bound = found_key;
+    const unsigned bound = max(found_key, kLowestKey);   // (with fewer than topk above -inf, the search below ends at 0)
 #pragma unroll
     for (int k = 0; k < kSampleVecs; ++k) {
       if (tid + k * kSampleThreads < nvec) {
@@ -168,7 +172,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_topk_kernel(const T* __
         if (lane == 0) found_key = key;
       }
       __syncthreads();
-      thr_key = found_key;
+      thr_key = max(found_key, kLowestKey);
       found = true;
     }
   }
@@ -189,18 +193,25 @@ __global__ __launch_bounds__(kSampleThreads) void sample_topk_kernel(const T* __
       }
       if (block_count(cnt, ired) >= topk) prefix = cand;
     }
-    thr_key = prefix;
+    thr_key = max(prefix, kLowestKey);
   }
 
+  const bool forced = mx == INFINITY;      // (uniform)
+  if (forced) thr_key = order_key(INFINITY);
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < kSampleVecs; ++k) {
     if (tid + k * kSampleThreads < nvec) {
       float e[8];
       v[k].get(e);
+      if (forced) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (order_key(e[j]) >= thr_key) s += __expf((e[j] - mx) * inv_temp);
+        for (int j = 0; j < 8; ++j) s += order_key(e[j]) >= thr_key ? 1.f : 0.f;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (order_key(e[j]) >= thr_key) s += __expf((e[j] - mx) * inv_temp);
+      }
     }
   }
   // exclusive prefix of s over the threads (thread order = walk order) and the total
@@ -258,8 +269,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_topk_kernel(const T* __
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (pick < 0 && order_key(e[j]) >= thr_key) {
-            last = i * 8 + j;
-            cum += __expf((e[j] - mx) * inv_temp);
+            const float w = forced ? 1.f : __expf((e[j] - mx) * inv_temp);
+            if (w > 0.f) last = i * 8 + j;
+            cum += w;
             if (cum > rest) pick = last;
           }
         }
