@@ -946,7 +946,8 @@ class LLM(nn.Module):
         64 / 128, or an MLA latent key of at most 128 columns) and prompt plus new tokens fit the context: a decode step is a few hundred small kernels, bound by launch cost.
 
         ``penalties``: keyword arguments of ``ops.penalize_logits`` (``repetition``, ``presence``, ``frequency``, ``bias``,
-        ``allowed``), applied to the logits of every step with the tokens so far as the history."""
+        ``allowed``), applied to the logits of every step with the tokens so far as the history. Where they leave a row no
+        token at all it gets token 0."""
         was_training = self.training
         self.eval()
         try:

@@ -13,14 +13,21 @@ from .._ext import ops, use_hip
 
 
 def sample_eager(logits: torch.Tensor, temperature: float = 1.0, topk: int | None = None) -> torch.Tensor:
-    """``logits [B, V]`` -> token ids ``[B, 1]`` with stock ops (no host-built index tensors)."""
+    """``logits [B, V]`` -> token ids ``[B, 1]`` with stock ops (no host-built index tensors). Tokens of -inf are never
+    drawn, those of +inf share the draw equally, and a row of nothing but -inf gives token 0."""
     logits = logits.float()
     if temperature > 0:
         logits = logits / temperature
     if topk is not None:
         v, _ = torch.topk(logits, min(topk, logits.size(-1)))
         logits = logits.masked_fill(logits < v[:, -1:], -float("inf"))
-    return torch.multinomial(F.softmax(logits, dim=-1), num_samples=1)
+    # The softmax of infinite logits has no value: it gets the largest numbers instead, and what is -inf is taken out of its
+    # result. The 1e-37 goes to token 0 and decides where nothing else is left. (No reduction over the row, here: over a
+    # long one torch clears its semaphores with a memset, which a captured step must not hold.)
+    most = torch.finfo(logits.dtype).max
+    p = F.softmax(logits.clamp(-most, most), dim=-1).masked_fill(logits == -float("inf"), 0.0)
+    p[:, :1] += 1e-37
+    return torch.multinomial(p, num_samples=1)
 
 
 def _fused_ok(logits: torch.Tensor) -> bool:
@@ -47,7 +54,8 @@ def sample_step(logits: torch.Tensor, temperature: float, topk: int | None, seed
 
 def sample_fused(logits: torch.Tensor, temperature: float = 1.0, topk: int | None = None,
                  seed: torch.Tensor | None = None) -> torch.Tensor:
-    """Same distribution from one kernel launch. ``seed``: int64 ``[1]`` on the device (default: drawn)."""
+    """Same distribution from one kernel launch, infinite logits included. ``seed``: int64 ``[1]`` on the device (default:
+    drawn)."""
     if not _fused_ok(logits):
         return sample_eager(logits, temperature, topk)
     if seed is None:
@@ -73,7 +81,8 @@ def penalize_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, pr
     * ``presence`` and ``frequency``: a token generated n > 0 times loses ``presence + n * frequency``;
     * ``bias`` (fp32 ``[V]`` or ``[R, V]``) is added;
     * ``allowed`` (int32 ``[ceil(V / 32)]`` or one such row per row of logits): tokens whose bit ``v % 32`` of word ``v // 32``
-      is clear become -inf, whatever their logit was. A row that allows nothing is -inf throughout.
+      is clear become -inf, whatever their logit was. A row that allows nothing is -inf throughout, and the samplers
+      give token 0 for it.
 
     The penalties are numbers or fp32 tensors with one value or one per row, lengths int32 tensors likewise; they are
     read by the kernel, so a captured step sees what a replay's buffers hold. ``out`` may be ``logits`` itself."""

@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from distributed_pytorch_amd import ops
+from distributed_pytorch_amd.config import LLMconfig
+from distributed_pytorch_amd.models.llm import LLM
 
 
 def masked_row(V, share, seed, device, dtype):
@@ -14,6 +16,60 @@ def masked_row(V, share, seed, device, dtype):
     ok = torch.rand(V, generator=g) < share
     ok[V // 3] = True
     return x.masked_fill(~ok, -math.inf).to(dtype).to(device), ok.to(device)
+
+
+def infinite_rows(V):
+    """Logits and the set that may be drawn: nothing allowed, one token, one and two forced by +inf, a plain row."""
+    x = torch.randn(5, V, generator=torch.Generator().manual_seed(3))
+    x[0] = -math.inf
+    x[1, 1:] = -math.inf
+    x[2, V - 1] = math.inf
+    x[2, : V // 2] = -math.inf
+    x[3, 5], x[3, V - 3] = math.inf, math.inf
+    return x, [{0}, {0}, {V - 1}, {5, V - 3}, set(range(V))]
+
+
+def check_infinite_rows(sample, V, device, dtype):
+    x, sets = infinite_rows(V)
+    x = x.to(dtype).to(device)
+    for topk in (None, 1, 2, 7, V):
+        seen = set()
+        for _ in range(30):
+            tok = sample(x, 0.7, topk)
+            assert tok.shape == (5, 1) and tok.dtype == torch.int64
+            for t, ok in zip(tok[:, 0].tolist(), sets):
+                assert t in ok
+            seen.add(int(tok[3]))
+        if topk != 1:
+            assert seen == sets[3]       # 30 draws of a fair coin: both, but for 2^-29
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_eager_sampler_on_rows_of_infinite_logits(dtype):
+    torch.manual_seed(0)
+    check_infinite_rows(ops.sample_eager, 64, "cpu", dtype)
+
+
+def test_eager_sampler_draws_what_it_drew():
+    """Finite logits: the same tokens as the plain chain from the same random numbers."""
+    x = torch.randn(50, 97, generator=torch.Generator().manual_seed(1)) * 3
+    for topk in (None, 1, 10, 200):
+        torch.manual_seed(4)
+        got = ops.sample_eager(x, 0.8, topk)
+        y = x / 0.8
+        if topk is not None:
+            y = y.masked_fill(y < torch.topk(y, min(topk, 97)).values[:, -1:], -math.inf)
+        torch.manual_seed(4)
+        assert torch.equal(got, torch.multinomial(torch.softmax(y, -1), 1))
+
+
+def test_generation_where_nothing_is_allowed():
+    m = LLM(LLMconfig(vocab_size=97, block_size=48, n_embd=32, n_layer=1, n_head=4, up_dim=48, attn="mha", pos_emb="learn",
+                      non_linearity="gelu").finalize()).eval()
+    none = dict(allowed=torch.zeros(4, dtype=torch.int32))
+    idx = torch.randint(1, 97, (2, 3))
+    assert (m.generate(idx, 5, penalties=none)[:, 3:] == 0).all()
+    assert all((o[3:] == 0).all() for o in m.generate_ragged(list(idx), 5, penalties=none))
 
 
 # ---- GPU ---------------------------------------------------------------------------------------------
@@ -52,3 +108,31 @@ def test_fused_sampler_on_masked_rows_follows_the_softmax(dtype, topk):
         # bound of five standard deviations does not hold here: many tokens expect less than one draw.)
         L, var = 30.0, rows * p * (1 - p)
         assert ((freq - p).abs() * rows <= L / 3 + (L * L / 9 + 2 * L * var).sqrt()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_samplers_on_rows_of_infinite_logits(dtype):
+    torch.manual_seed(0)
+    for V in (64, 8200):
+        check_infinite_rows(ops.sample_fused, V, "cuda", dtype)
+        check_infinite_rows(ops.sample_eager, V, "cuda", dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_generation_under_a_mask_on_the_gpu(graph):
+    """Dense and ragged generation, eager and captured: allowed tokens only, and token 0 where none is allowed."""
+    torch.manual_seed(0)
+    m = LLM(LLMconfig(vocab_size=512, block_size=256, n_embd=256, n_layer=2, n_head=4, up_dim=512, attn="mha", pos_emb="learn",
+                      non_linearity="gelu").finalize()).cuda().to(torch.bfloat16).eval()
+    idx = torch.randint(1, 512, (4, 9), device="cuda")
+    some = torch.zeros(16, dtype=torch.int32, device="cuda")
+    some[3], some[9] = 0b1010, 1
+    for allowed, may in ((some, {97, 99, 288}), (torch.zeros_like(some), {0})):
+        for topk in (None, 50):
+            pen = dict(allowed=allowed)
+            out = m.generate(idx, 40, topk=topk, hip_graph=graph, penalties=pen)
+            assert m.last_decode_graphed == graph and set(out[:, 9:].unique().tolist()) <= may
+            out = m.generate_ragged(list(idx), 40, topk=topk, hip_graph=graph, penalties=pen)
+            assert m.last_decode_graphed == graph and set(torch.stack(out)[:, 9:].unique().tolist()) <= may
