@@ -12,6 +12,7 @@
 
 #include "mfma_tiles.h"
 #include "paged.h"
+#include "paged_items.h"
 
 namespace dpa {
 
@@ -138,8 +139,8 @@ __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAt
 // Scores are scaled in fp32 after the product: q keeps its bits. A negative scale negates q, which is exact.
 // ---------------------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFewRows = 32, kChunkRows = 128, kThreads = 256;
-constexpr int kFewStep = 128, kChunkStep = 64;      // keys a workgroup advances by: pieces are multiples of it
+using namespace paged;
+constexpr int kThreads = 256;
 
 template <typename T> struct Frag;
 template <> struct Frag<bf16_t> {
@@ -166,8 +167,6 @@ template <> struct Frag<half_t> {
   }
 };
 
-constexpr int kWaveRequests = 256;    // up to here every wave derives the items by itself
-
 struct FastArgs {
   float c;             // |scale| log2 e
   bool negate;         // scale < 0
@@ -179,57 +178,12 @@ struct FastArgs {
   float* part;         // [max_slots][slot_rows][W] unnormalised outputs of pieces
   float* ml;           // [max_slots][slot_rows][2] reference, sum
   int* meta;           // [max_slots][8]
-  int* header;         // [0] = slots in use, [1], [2] = keys per piece
+  int* header;         // [0] = slots in use, [1], [2] = keys per piece (R > kWaveRequests), [3] = cu_q decreases
   int* prefix;         // R > kWaveRequests: [3][R + 1] first items (few rows: steps), slots and second items before each request
 };
 
 // 256 zero bytes: what rows that no query may see, and pages that do not exist, read as
 __device__ __attribute__((aligned(256))) const unsigned zero_row[64] = {};
-
-struct Request {
-  int start, n;        // its rows of the batch
-  int shift;           // position of batch row i: i + shift
-  int rows, tiles;     // packed rows per KV head and tiles of them
-  int klo, khi;        // keys that any of its rows sees
-  bool chunk;
-};
-__device__ __forceinline__ void key_range(const PagedAttnArgs& a, Request& q) {
-  q.klo = a.window > 0 ? max(q.start + q.shift - a.window + 1, 0) : 0;
-  q.khi = max(min(q.start + q.n + q.shift, a.M * a.page), q.klo);
-}
-__device__ __forceinline__ Request request(const PagedAttnArgs& a, const FastArgs& f, int r) {
-  Request q;
-  const int c0 = a.cu_q[r], c1 = a.cu_q[r + 1];
-  q.start = min(max(c0, 0), a.N);
-  q.n = min(max(c1, q.start), a.N) - q.start;
-  const long long sh = (long long)a.kv_lens[r] - c1;
-  q.shift = (int)min(max(sh, -(1ll << 30)), 1ll << 30);
-  q.rows = q.n * f.G;
-  q.chunk = q.rows > kFewRows;
-  q.tiles = q.chunk ? (q.rows + kChunkRows - 1) / kChunkRows : (q.rows > 0 ? 1 : 0);
-  key_range(a, q);
-  return q;
-}
-
-// Work of a request: keys walked by a workgroup, those of a chunk counted twice (its steps have 64 keys, those of few
-// rows 128).
-__device__ __forceinline__ float request_cost(const Request& q) {
-  return (float)q.tiles * (float)(q.khi - q.klo) * (q.chunk ? 2.f : 1.f);
-}
-struct PieceSize {
-  int few, chunk;      // keys
-};
-__device__ __forceinline__ PieceSize piece_size(float cost, int nkv, int target) {
-  const float budget = cost * (float)nkv / (float)target;
-  PieceSize p;
-  p.few = max((int)fminf(budget / (float)kFewStep, 8e6f) + 1, 2) * kFewStep;
-  p.chunk = max((int)fminf(budget * 0.5f / (float)kChunkStep, 8e6f) + 1, 8) * kChunkStep;
-  return p;
-}
-__device__ __forceinline__ int pieces(const Request& q, const PieceSize& p) {
-  const int len = q.khi - q.klo, step = q.chunk ? p.chunk : p.few;
-  return len <= step ? 1 : (len + step - 1) / step;
-}
 
 // Inclusive prefix sum over the wave by register moves between lanes (shifts inside rows of 16, then row broadcasts).
 __device__ __forceinline__ int wave_scan(int x) {
@@ -285,15 +239,20 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
     constexpr int PER = kWaveRequests / 64;      // consecutive requests per lane
     Request q[PER];
     float cost = 0.f;
+    bool back = false;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       q[u].tiles = 0;
       const int per = (a.R + 63) >> 6, r = lane * per + u;
       if (u < per && r < a.R) {
-        q[u] = request(a, f, r);
+        q[u] = request(a, f.G, r);
         cost += request_cost(q[u]);
+        back |= q[u].back;
       }
     }
+    const int any_back = __any(back);
+    if (id == 0) f.header[3] = any_back;
+    if (any_back) return it;
     const PieceSize size = piece_size(wave_total(cost), a.nkv, f.target);
     int items[PER], ahead[PER], slots[PER], n1 = 0, n2 = 0, ns = 0;
 #pragma unroll
@@ -301,8 +260,8 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
       items[u] = ahead[u] = slots[u] = 0;
       if (q[u].tiles > 0) {
         const int np = pieces(q[u], size);
-        ahead[u] = (q[u].tiles - q[u].tiles / 3) * np * a.nkv;
-        items[u] = q[u].tiles / 3 * np * a.nkv;
+        ahead[u] = first_items(q[u], np, a.nkv);
+        items[u] = second_items(q[u], np, a.nkv);
         slots[u] = np > 1 ? ahead[u] + items[u] : 0;
       }
       n1 += ahead[u];
@@ -346,6 +305,7 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
     it.np = __builtin_amdgcn_readlane(np, src);
     return it;
   }
+  if (f.header[3] != 0) return it;
   const int* const second = f.prefix + 2 * (a.R + 1);
   const int all1 = f.prefix[a.R];
   const int lo = id < all1 ? find_prefix(f.prefix, a.R, id, lane) : find_prefix(second, a.R, id - all1, lane);
@@ -353,7 +313,7 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
   it.r = lo;
   it.j = id < all1 ? id - f.prefix[lo] : f.prefix[lo + 1] - f.prefix[lo] + id - all1 - second[lo];
   it.slot = f.prefix[a.R + 1 + lo] + it.j;
-  const Request q = request(a, f, lo);
+  const Request q = request(a, f.G, lo);
   PieceSize size;
   size.few = f.header[1];
   size.chunk = f.header[2];
@@ -366,26 +326,24 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
 // takes steps [i * per, (i + 1) * per) of them all, whichever runs they fall into: contexts of any mix of lengths load
 // the card evenly in one round. At most its first and its last run are cut.
 constexpr int kMinSteps = 1;           // steps worth a workgroup of their own (8 x 1k keys: 17.2 us; 2: 19.7, 4: 20.9, 8, uncut: 31.7)
-__device__ __forceinline__ int run_base(const Request& q) { return q.klo & ~31; }
-__device__ __forceinline__ int run_steps(const Request& q) {
-  return q.rows > 0 ? max((q.khi - run_base(q) + kFewStep - 1) / kFewStep, 1) : 0;
-}
-__device__ __forceinline__ int run_count(const Request& q, int nkv) { return (q.rows + kFewRows - 1) / kFewRows * nkv; }
 
 struct Runs {        // the requests of the batch in LDS (R <= kWaveRequests)
   int before[kWaveRequests + 1];       // steps before each
   int start[kWaveRequests], rows[kWaveRequests], shift[kWaveRequests];
   int red[kThreads / 64];
+  int back[kThreads / 64];
 };
 static_assert(kWaveRequests == kThreads, "one request per thread");
-// Steps of all runs; leaves `runs` filled for every thread.
+// Steps of all runs, none if cu_q decreases; leaves `runs` filled for every thread.
 __device__ __forceinline__ int list_runs(const PagedAttnArgs& a, const FastArgs& f, Runs& runs) {
-  if (a.R > kWaveRequests) return f.prefix[a.R];
+  if (a.R > kWaveRequests) return f.header[3] != 0 ? 0 : f.prefix[a.R];
   const int tid = threadIdx.x;
   int steps = 0;
+  bool back = false;
   if (tid < a.R) {
-    const Request q = request(a, f, tid);
+    const Request q = request(a, f.G, tid);
     steps = run_steps(q) * run_count(q, a.nkv);
+    back = q.back;
     runs.start[tid] = q.start;
     runs.rows[tid] = q.rows;
     runs.shift[tid] = q.shift;
@@ -400,8 +358,12 @@ __device__ __forceinline__ int list_runs(const PagedAttnArgs& a, const FastArgs&
   }
   if (tid < a.R) runs.before[tid + 1] = incl;
   if (tid == 0) runs.before[0] = 0;
+  const int any_back = __any(back);
+  if ((tid & 63) == 0) runs.back[tid >> 6] = any_back;
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(runs.before[a.R]);
+  const int bad = runs.back[0] | runs.back[1] | runs.back[2] | runs.back[3];
+  if (blockIdx.x == 0 && tid == 0) f.header[3] = bad;
+  return __builtin_amdgcn_readfirstlane(bad != 0 ? 0 : runs.before[a.R]);
 }
 // The request of step `at`, and the number of its first step; r < 0: there is none.
 __device__ __forceinline__ int find_run(const PagedAttnArgs& a, const FastArgs& f, const Runs& runs, int at, int& first, Request& q) {
@@ -410,7 +372,7 @@ __device__ __forceinline__ int find_run(const PagedAttnArgs& a, const FastArgs& 
     const int r = find_prefix(f.prefix, a.R, at, lane);
     if (r < 0) return -1;
     first = __builtin_amdgcn_readfirstlane(f.prefix[r]);
-    q = request(a, f, r);
+    q = request(a, f.G, r);
     return r;
   }
   int below = 0;
@@ -433,20 +395,26 @@ __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a,
   __shared__ int red_i[16], red_s[16], red_2[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float cost = 0.f;
-  if (CHUNKS) {
-    for (int r = tid; r < a.R; r += 1024) cost += request_cost(request(a, f, r));
-    cost = block_sum(cost, red_f);
+  bool back = false;
+  for (int r = tid; r < a.R; r += 1024) {
+    const Request q = request(a, f.G, r);
+    if (CHUNKS) cost += request_cost(q);
+    back |= q.back;
   }
+  if (CHUNKS) cost = block_sum(cost, red_f);
+  back = __syncthreads_or(back);
+  if (tid == 0) f.header[3] = back;
+  if (back) return;
   const PieceSize size = piece_size(cost, a.nkv, f.target);
   int base_i = 0, base_s = 0, base_2 = 0;
   for (int r0 = 0; r0 < a.R; r0 += 1024) {
     const int r = r0 + tid;
     int ni = 0, ns = 0, n2 = 0;
     if (r < a.R) {
-      const Request q = request(a, f, r);
+      const Request q = request(a, f.G, r);
       const int np = CHUNKS ? pieces(q, size) : 1;
-      ni = CHUNKS ? (q.tiles - q.tiles / 3) * np * a.nkv : run_steps(q) * run_count(q, a.nkv);
-      n2 = CHUNKS ? q.tiles / 3 * np * a.nkv : 0;
+      ni = CHUNKS ? first_items(q, np, a.nkv) : run_steps(q) * run_count(q, a.nkv);
+      n2 = CHUNKS ? second_items(q, np, a.nkv) : 0;
       ns = np > 1 ? ni + n2 : 0;
     }
     int pi = wave_scan(ni), ps = wave_scan(ns), p2 = wave_scan(n2);
@@ -1101,8 +1069,10 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const FastArgs&
   }
 }
 
-__device__ __forceinline__ void zero_rows_outside(const PagedAttnArgs& a) {
-  const int lo = a.R > 0 ? min(max(a.cu_q[0], 0), a.N) : a.N, hi = a.R > 0 ? min(max(a.cu_q[a.R], 0), a.N) : a.N;
+// `all`: cu_q says nothing about which rows belong to a request.
+__device__ __forceinline__ void zero_rows_outside(const PagedAttnArgs& a, bool all = false) {
+  const bool none = all || a.R == 0;
+  const int lo = none ? a.N : min(max(a.cu_q[0], 0), a.N), hi = none ? a.N : min(max(a.cu_q[a.R], 0), a.N);
   const int rest = lo + a.N - max(hi, lo);
   const long long total = (long long)rest * a.nh * a.width;
   for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
@@ -1153,7 +1123,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kern
     if (steps == 0) break;
     const int run = (at - first) / steps, s0 = at - first - run * steps, s1 = min(steps, s0 + end - at);
     const int g = run % a.nkv, rows0 = run / a.nkv * kFewRows;
-    if (s0 < 0 || run < 0 || rows0 >= q.rows) break;   // lengths that contradict each other
+    if (s0 < 0 || run < 0 || rows0 >= q.rows) break;   // (count_items' bounds: never)
     const Tile t = make_tile(a, f, q, r, g, rows0, kFewRows);
     const int base = run_base(q), k0 = base + s0 * kFewStep, k1 = min(t.khi, base + s1 * kFewStep);
     const bool whole = s0 == 0 && s1 == steps;
@@ -1234,7 +1204,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? (RUN > 0 ? 4 : 3) : 2) void pag
   const Item it = find_item(a, f, blockIdx.x, lane);
   const int r = __builtin_amdgcn_readfirstlane(it.r);
   if (r < 0) return;
-  const Request q = request(a, f, r);
+  const Request q = request(a, f.G, r);
   const int np = __builtin_amdgcn_readfirstlane(it.np);
   int slot = __builtin_amdgcn_readfirstlane(it.slot);
   int j = __builtin_amdgcn_readfirstlane(it.j);
@@ -1242,7 +1212,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? (RUN > 0 ? 4 : 3) : 2) void pag
   j /= a.nkv;
   const int piece = j % np;
   const int tile = q.tiles - 1 - j / np;                 // the rows that see most come first
-  if (tile < 0 || j < 0 || (np > 1 && (unsigned)slot >= (unsigned)f.max_slots)) return;   // lengths that contradict each other
+  if (tile < 0 || j < 0 || (np > 1 && (unsigned)slot >= (unsigned)f.max_slots)) return;   // (count_items' bounds: never)
   const int rows0 = tile * kChunkRows;
   const Tile t = make_tile(a, f, q, r, g, rows0, q.chunk ? kChunkRows : kFewRows);
   const int nrows = t.nrows, step = q.chunk ? kChunkStep : kFewStep;
@@ -1304,11 +1274,15 @@ __global__ __launch_bounds__(kThreads) void paged_attn_join_kernel(PagedAttnArgs
   constexpr int CPR = W / 8, kJoinRows = kThreads / CPR, U = 4;
   __shared__ float o_s[kThreads][9], m_s[kThreads];      // (9: rows of 8 floats would share banks)
   const int slot = blockIdx.x;
+  if (f.header[3] != 0) {       // nothing was computed
+    if (a.zero_rest) zero_rows_outside(a, true);
+    return;
+  }
   if (slot >= f.header[0]) return;
   const int* meta = f.meta + (long long)slot * 8;
   const int np = meta[0], start = meta[1], rows0 = meta[2], nrows = min(meta[3] - (int)blockIdx.y * kJoinRows, kJoinRows), g = meta[4];
   const int other = meta[5], stride = meta[6];
-  if (np < 2 || nrows <= 0 || other + (np - 1) * stride >= f.max_slots) return;      // (lengths that contradict each other)
+  if (np < 2 || nrows <= 0 || other + (np - 1) * stride >= f.max_slots) return;
   const int row_b = blockIdx.y * kJoinRows, units = nrows * CPR;
   int groups = 1;
   while (2 * groups * units <= kThreads) groups *= 2;
@@ -1383,30 +1357,12 @@ bool fast_ok(const PagedAttnArgs& a) {
   return a.k_rs * 2 * std::max(a.page, 16) < lim && a.v_rs * 2 * std::max(a.page, 16) < lim && a.k_ps * 2 < lim && a.v_ps * 2 < lim;
 }
 
-struct Plan {
-  int target, grid, slots, slot_rows;
-  bool chunks;
+struct Plan : Counts {
   size_t part, ml, meta, total;
 };
 Plan plan_items(const PagedAttnArgs& a, int num_cus) {
-  Plan p;
-  const int W = a.width <= 64 ? 64 : 128, G = a.nh / a.nkv;
-  // (the 128-key steps of all runs are counted in 32 bits; pages shared by many long requests could pass that)
-  const long long steps = (a.R + (long long)a.N * G / kFewRows) * a.nkv * ((long long)a.M * a.page / kFewStep + 2);
-  p.chunks = ((long long)a.N * G > kFewRows && (long long)a.max_q * G > kFewRows) || steps >= (1ll << 31);
-  if (p.chunks) {
-    p.target = num_cus * 2;         // (4: 43 instead of 37 us on a mixed batch of 33 requests, no difference on prompts)
-    // tiles: one per request with rows, and one more for every 128 rows of a chunk
-    const long long tiles = std::min<long long>(a.N, a.R) + (long long)a.N * G / kChunkRows;
-    p.grid = (int)std::min<long long>(p.target + tiles * a.nkv, 1ll << 30);
-    p.slots = (int)std::min<long long>(2ll * p.target, p.grid);
-    p.slot_rows = kChunkRows;
-  } else {
-    p.target = 0;
-    p.grid = num_cus * (W == 64 ? 3 : 2);      // the workgroups that fit the card at once
-    p.slots = 2 * p.grid;
-    p.slot_rows = kFewRows;
-  }
+  Plan p{count_items(a, num_cus)};
+  const int W = a.width <= 64 ? 64 : 128;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.part = up((size_t)p.slots * p.slot_rows * W * 4);
   p.ml = up((size_t)p.slots * p.slot_rows * 8);

@@ -122,7 +122,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """``q [N, nh, width]``, the newest tokens of every request (rows ``cu_q[r] .. cu_q[r + 1]``), over the request's
     ``kv_lens[r]`` cached rows, their own among them: the request's last row sees all of them, each row before it one
     less, and with ``window`` only the newest ``window`` of those. Grouped-query heads as in ``causal_attention``. A row
-    without any key gives zeros; keys whose table entry names no page of the pool are left out.
+    without any key gives zeros; keys whose table entry names no page of the pool are left out. ``cu_q`` must not decrease:
+    what the rows then hold is unspecified (nothing outside the buffers is touched).
 
     ``max_q``: an upper bound of the new tokens of a request, if the host knows one (a decode step: 1); it selects
     kernels, not results. ``out``: the result's buffer; rows outside every request keep what it holds (without

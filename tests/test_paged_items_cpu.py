@@ -1,0 +1,21 @@
+"""The work lists of paged attention on the host, under AddressSanitizer + UBSan (CPU only)."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_every_slot_that_is_joined_has_been_written(tmp_path):
+    """Also for offsets that decrease or leave the batch, and lengths outside the table."""
+    exe = tmp_path / "paged_items_checks"
+    build = subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                            "-static-libasan", "-static-libubsan", "-I", os.path.join(ROOT, "csrc"),
+                            os.path.join(ROOT, "tests", "native", "paged_items_checks.cpp"), "-o", str(exe)],
+                           capture_output=True, text=True)
+    assert build.returncode == 0, build.stderr[-4000:]
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "paged item checks passed" in run.stdout, (run.stdout + run.stderr)[-4000:]
