@@ -49,12 +49,13 @@ DPA_HD float request_cost(const Request& q) { return (float)q.tiles * (float)(q.
 struct PieceSize {
   int few, chunk;      // keys
 };
+// (the limits are 2.05e9 keys, past the 2^30 of the longest request: what they cut is one piece)
 DPA_HD PieceSize piece_size(float cost, int nkv, int target) {
   const float budget = cost * (float)nkv / (float)target;
   const float few = budget / (float)kFewStep, chunk = budget * 0.5f / (float)kChunkStep;
   PieceSize p;
-  p.few = imax((int)(few < 8e6f ? few : 8e6f) + 1, 2) * kFewStep;
-  p.chunk = imax((int)(chunk < 8e6f ? chunk : 8e6f) + 1, 8) * kChunkStep;
+  p.few = imax((int)(few < 1.6e7f ? few : 1.6e7f) + 1, 2) * kFewStep;
+  p.chunk = imax((int)(chunk < 3.2e7f ? chunk : 3.2e7f) + 1, 8) * kChunkStep;
   return p;
 }
 DPA_HD int pieces(const Request& q, const PieceSize& p) {

@@ -162,6 +162,17 @@ int main() {
     f.max_q = 1;                           // a hint that is too small selects the other list, with all rows
     if (!count_items(f, kCus).chunks) few_list(f);
   }
+  // the longest requests that the arguments allow, many of them: no piece is lost to the limits of the piece sizes
+  {
+    std::vector<int> cu(1001), kv(1000, (1 << 30) - 1);
+    for (int i = 0; i <= 1000; ++i) cu[i] = i;
+    Batch b = batch(cu, kv, 1000, 8, 8, (1 << 30) - (1 << 20), 1 << 20, 0, 1);
+    CHECK(count_items(b, kCus).chunks);
+    CHECK(chunk_list(b, true) == 0);
+    for (int i = 0; i <= 1000; ++i) cu[i] = 40 * i;
+    b = batch(cu, kv, 40000, 8, 8, (1 << 30) - (1 << 20), 1 << 20, 0, 40);
+    CHECK(chunk_list(b, true) == 0);
+  }
   if (g_failed) return 1;
   std::puts("paged item checks passed");
   return 0;
