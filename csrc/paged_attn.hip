@@ -134,8 +134,11 @@ __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAt
 // vector-memory wait, which waits for the transfers in flight: 737 -> 1232 us on the prompts), so what is rare is done
 // elsewhere (exact_rows); and no register that an ordinary load fills may have its first use in them (load_row).
 //
-// The score's reference point mb (log2 units) moves only when a subtile's maximum passes it by 2^8: p <= 2^(kBias + 8).
-// kBias = 6 for fp16 keeps small probabilities out of its subnormal range (one of 2^-20 still has all its bits).
+// The score's reference point mb (log2 units) does not follow every new maximum. Few rows move it when a subtile's
+// maximum passes mb + kBias + 8, chunks when 16 keys sum to more than kSumMax: p <= 2^8 for bf16 either way, 2^14 (few
+// rows) or 2^15 (chunks) for fp16. kBias = 6 for fp16 keeps small probabilities out of its subnormal range (one of 2^-20
+// still has all its bits). The output is divided by the sum at the end, so 2^8 |v| times the number of keys has to stay
+// below fp32's 3.4e38: bf16 values up to 1e30 with 2^20 keys and a reference as far off as it gets.
 // Scores are scaled in fp32 after the product: q keeps its bits. A negative scale negates q, which is exact.
 // ---------------------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
@@ -732,7 +735,7 @@ __device__ __forceinline__ bool chunk_tile(const char* kt, const char* vt, int k
                                            RowState<W>& st, int lane) {
   typedef Frag<T> F;
   constexpr int NK = W / 16, ND = W / 32;
-  constexpr float kSumMax = F::kBias ? 32768.f : 1.0e9f;
+  constexpr float kSumMax = F::kBias ? 32768.f : 256.f;
   const int r = lane & 31, hh = lane >> 5;
   f32x16 s;
   auto scores = [&]() {
