@@ -140,7 +140,12 @@ class PagedKVCache:
 
     Per layer a pool ``k[i], v[i] [pages, page_size, n_kv_heads, head_size]``; the table, the lengths and the free list
     are device tensors (``ops/paged.py``), so a step has no host-side shape but its number of rows and can be captured.
-    A step: ``begin(q_lens, num_tokens)``, a forward of the packed tokens ``[1, num_tokens]``, ``commit()``."""
+    A step: ``begin(q_lens, num_tokens)``, a forward of the packed tokens ``[1, num_tokens]``, ``commit()``.
+
+    ``free_left`` (int32 ``[2]``): pages on the free list, and pages that all steps so far asked for in vain, because the list
+    was empty or the table full. Tokens without a page are not in the cache, so once the second is not 0 the requests'
+    later tokens attend over a context with holes; a serving loop looks at it whenever it reads anything back. Pages stay
+    with their request: there is no way to hand a finished one's back."""
 
     def __init__(self, config: LLMconfig, requests: int, max_len: int, pages: int, device, dtype, page_size: int = 16):
         if config.attn not in ("mha", "mqa", "gqa"):
@@ -155,7 +160,8 @@ class PagedKVCache:
         self.table = torch.full((requests, columns), -1, dtype=torch.int32, device=device)
         self.ctx_lens = torch.zeros(requests, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(pages, dtype=torch.int32, device=device)
-        self.free_left = torch.tensor([pages, 0], dtype=torch.int32, device=device)   # [1]: pages a step asked for in vain
+        self.free_left = torch.tensor([pages, 0], dtype=torch.int32, device=device)
+        self._carry = torch.tensor([0, 1], dtype=torch.int32, device=device)     # what a step leaves of free_left
         self.plan = None
         self.max_q = None
 
@@ -166,7 +172,7 @@ class PagedKVCache:
 
     def commit(self):
         self.ctx_lens.copy_(self.plan.kv_lens)
-        self.free_left.copy_(self.plan.free_left)
+        torch.addcmul(self.plan.free_left, self.free_left, self._carry, out=self.free_left)
 
     def layer(self, i: int):
         return _PagedLayer(self.k[i], self.v[i], self)
