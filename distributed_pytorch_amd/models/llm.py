@@ -866,7 +866,8 @@ class LLM(nn.Module):
             # packed tokens of a ragged batch: every row has a position of its own, gathered on the device
             assert B == 1 and targets is None, "paged cache: the requests' tokens in one row, no targets"
             paged = kv_caches
-            at = paged.plan.positions
+            # (a request past the context is the caller's mistake, but the tables end there: its tokens read their last row)
+            at = paged.plan.positions.clamp(max=cfg.block_size - 1)
             ptab = self._pos_table(wte.dtype, wte.device)
             x = ops.embedding(idx, wte, None if ptab is None else ptab.index_select(0, at), 0)
             rope = None

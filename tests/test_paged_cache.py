@@ -38,3 +38,20 @@ def test_a_shortage_of_pages_is_not_forgotten(device):
         assert cache.free_left.tolist() == [0, 1]
     step(m, cache, [1], [3])
     assert cache.free_left.tolist() == [0, 2] and cache.ctx_lens.tolist() == [13]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("pos_emb", ["learn", "sin", "rope"])
+def test_steps_past_the_context_stay_inside_the_position_tables(device, pos_emb):
+    """Lengths are not known to the host, so nothing refuses such a step: it must not read past the tables."""
+    m = small(device, pos_emb=pos_emb, block_size=16)
+    cache = PagedKVCache(m.config, 2, 16, 8, device, torch.float32, 8)
+    step(m, cache, [16, 1], list(range(17)))
+    inside = step(m, cache, [0, 1], [5])[1]
+    both = step(m, cache, [3, 1], [7, 8, 9, 5])
+    assert cache.ctx_lens.tolist() == [19, 3] and cache.free_left.tolist() == [8 - 3, 1]
+    assert torch.isfinite(both).all() and torch.isfinite(inside).all()
+    # the request that kept inside is not disturbed
+    alone = PagedKVCache(m.config, 1, 16, 8, device, torch.float32, 8)
+    want = step(m, alone, [3], [16, 5, 5])
+    assert torch.allclose(both[1], want[0], rtol=1e-4, atol=1e-5)
