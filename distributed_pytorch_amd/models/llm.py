@@ -140,7 +140,9 @@ class PagedKVCache:
 
     Per layer a pool ``k[i], v[i] [pages, page_size, n_kv_heads, head_size]``; the table, the lengths and the free list
     are device tensors (``ops/paged.py``), so a step has no host-side shape but its number of rows and can be captured.
-    A step: ``begin(q_lens, num_tokens)``, a forward of the packed tokens ``[1, num_tokens]``, ``commit()``.
+    A step: ``begin(q_lens, num_tokens)``, a forward of the packed tokens ``[1, num_tokens]``, ``commit()``. The forward
+    gives the logits ``[requests, 1, V]`` of every request's newest token; a request without new tokens has none, its
+    row is zero.
 
     ``free_left`` (int32 ``[2]``): pages on the free list, and pages that all steps so far asked for in vain, because the list
     was empty or the table full. Tokens without a page are not in the cache, so once the second is not 0 the requests'
@@ -924,9 +926,10 @@ class LLM(nn.Module):
                                                      expected_grad=self.loss_grad_scale if self.training else 1.0)
             loss = main_loss + total_aux / cfg.n_layer
         elif paged is not None:
-            # the newest row of every request: logits [requests, 1, V]
-            last = (paged.plan.cu_q[1:] - 1).clamp_(min=0)
-            logits = ops.linear(x[0].index_select(0, last)[:, None, :], wte)
+            # the newest row of every request: logits [requests, 1, V], zeros for a request without new tokens
+            cu = paged.plan.cu_q
+            h = x[0].index_select(0, (cu[1:] - 1).clamp_(min=0)).masked_fill_((cu[1:] <= cu[:-1])[:, None], 0.0)
+            logits = ops.linear(h[:, None, :], wte)
             loss = None
         else:
             logits = ops.linear(x[:, -1:, :], wte)   # a slice, not a list index: no host-built index tensor

@@ -55,3 +55,18 @@ def test_steps_past_the_context_stay_inside_the_position_tables(device, pos_emb)
     alone = PagedKVCache(m.config, 1, 16, 8, device, torch.float32, 8)
     want = step(m, alone, [3], [16, 5, 5])
     assert torch.allclose(both[1], want[0], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_requests_without_new_tokens_have_no_logits(device):
+    """Their rows are zero, not another request's logits: at the front, between others and at the end."""
+    m = small(device)
+    cache = PagedKVCache(m.config, 4, 20, 20, device, torch.float32, 4)
+    first = step(m, cache, [0, 3, 0, 2], [1, 2, 3, 4, 5, 0, 0])       # two rows of padding
+    assert (first[[0, 2]] == 0).all()
+    with torch.no_grad():
+        for r, tokens in ((1, [1, 2, 3]), (3, [4, 5])):
+            want = m(torch.tensor([tokens], device=device))[0][0, -1]
+            assert torch.allclose(first[r, 0], want, rtol=1e-4, atol=1e-4)
+    then = step(m, cache, [2, 0, 1, 0], [6, 7, 8])
+    assert (then[[1, 3]] == 0).all() and (then[[0, 2]] != 0).any(-1).all()
