@@ -60,3 +60,10 @@ def use_hip(*tensors: torch.Tensor) -> bool:
         return False
     require()
     return True
+
+
+def refuse_grad(name: str, *tensors) -> None:
+    """For kernels without a backward pass: an error where autograd would have to record the call (it would lose the
+    gradient without a word, or with a warning)."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient on the GPU: call it under torch.no_grad() or on detached tensors")

@@ -849,6 +849,9 @@ class LLM(nn.Module):
         return None
 
     def forward(self, idx: torch.Tensor, targets=None, kv_caches=None):
+        if isinstance(kv_caches, PagedKVCache) and torch.is_grad_enabled():
+            with torch.no_grad():                       # its operators have no gradients
+                return self.forward(idx, targets, kv_caches)
         cfg = self.config
         B, T = idx.shape
         wte = self.lm_head.weight

@@ -10,7 +10,8 @@ A step is
     o = paged_attention(q, k_pages, v_pages, block_table, plan.cu_q, plan.kv_lens)               # per layer
 
 Lengths, tables and slots are int32 in device memory and never read by the host, so a step can be captured in a
-hipGraph whose replays see growing requests. No gradients.
+hipGraph whose replays see growing requests. No gradients: on the GPU, tensors that require them are refused outside
+``torch.no_grad()``.
 
 GPU: ``csrc/paged_plan.hip``, ``paged_append.hip``, ``paged_attn.hip`` (bf16, fp16, fp32). CPU: stock ops.
 Replaces, for ragged batches, the per-batch cache the reference grows by concatenation and its attention over it
@@ -23,7 +24,7 @@ from typing import NamedTuple
 
 import torch
 
-from .._ext import ops, use_hip
+from .._ext import ops, refuse_grad, use_hip
 
 _MAX_WIDTH = 256
 
@@ -100,6 +101,7 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
     ``[0, P * page)`` are skipped; the others must be distinct. Key and value widths may differ; the new rows lie outside
     the pools."""
     if use_hip(k_pages, k):
+        refuse_grad("paged_append", k_pages, v_pages, k, v)
         ops().paged_append(k_pages, v_pages, k, v, slots)
         return
     _check(k_pages.dim() == 4 and v_pages.dim() == 4 and k_pages.shape[:3] == v_pages.shape[:3],
@@ -132,6 +134,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         scale = 1.0 / math.sqrt(q.shape[-1])
     _check(window is None or window >= 1, "paged_attention: window must be positive or None")
     if use_hip(q, k_pages):
+        refuse_grad("paged_attention", q, k_pages, v_pages, out)
         o = ops().paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, scale, window or 0, max_q or 0, out)
         return o if out is None else out
     return paged_attention_eager(q, k_pages, v_pages, block_table, cu_q, kv_lens, scale, window, out)

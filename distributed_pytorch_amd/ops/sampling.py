@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from .._ext import ops, use_hip
+from .._ext import ops, refuse_grad, use_hip
 
 
 def sample_eager(logits: torch.Tensor, temperature: float = 1.0, topk: int | None = None) -> torch.Tensor:
@@ -85,8 +85,10 @@ def penalize_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, pr
       give token 0 for it.
 
     The penalties are numbers or fp32 tensors with one value or one per row, lengths int32 tensors likewise; they are
-    read by the kernel, so a captured step sees what a replay's buffers hold. ``out`` may be ``logits`` itself."""
+    read by the kernel, so a captured step sees what a replay's buffers hold. ``out`` may be ``logits`` itself. No
+    gradients: on the GPU, tensors that require them are refused outside ``torch.no_grad()``."""
     if use_hip(logits):
+        refuse_grad("penalize_logits", logits, repetition, presence, frequency, bias, out)
         rep, rep_v = _row_value(repetition, logits)
         pres, pres_v = _row_value(presence, logits)
         freq, freq_v = _row_value(frequency, logits)
