@@ -7,6 +7,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include "overlap.h"
+
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -1302,6 +1304,12 @@ void check_pages(const Tensor& t, const char* who, const char* name) {
   TORCH_CHECK(t.size(0) * t.size(1) < (int64_t(1) << 31), who, ": more than 2^31 rows in ", name);
 }
 
+// Refuses operands that share memory, also where both are strided (at::assert_no_overlap looks at dense ones only).
+void check_apart(const Tensor& a, const Tensor& b, const char* who, const char* names) {
+  auto block = [](const Tensor& t) { return dpa::Block(t.data_ptr(), t.sizes(), t.strides(), (int)t.dim(), t.element_size()); };
+  TORCH_CHECK(a.numel() == 0 || b.numel() == 0 || share(block(a), block(b)) != dpa::Share::kOverlap, who, ": ", names, " share memory");
+}
+
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_plan(const Tensor& q_lens, const Tensor& ctx_lens, Tensor table,
                                                               const Tensor& free_pages, const Tensor& free_count,
                                                               int64_t page, int64_t tokens) {
@@ -1372,10 +1380,10 @@ void paged_append(Tensor k_pages, Tensor v_pages, const Tensor& k, const Tensor&
   paged_type(k_pages, who);
   at::assert_no_internal_overlap(k_pages);
   at::assert_no_internal_overlap(v_pages);
-  at::assert_no_overlap(k_pages, v_pages);
+  check_apart(k_pages, v_pages, who, "the pools");
   for (const Tensor* t : {&k, &v}) {
-    at::assert_no_overlap(k_pages, *t);
-    at::assert_no_overlap(v_pages, *t);
+    check_apart(k_pages, *t, who, "new rows and k_pages");
+    check_apart(v_pages, *t, who, "new rows and v_pages");
   }
   check_int_vec(slots, k.size(0), k_pages, who, "slots");
   TORCH_CHECK(k.size(0) < (1 << 24) && page <= (1 << 20) && H * (k.size(2) + v.size(2)) < (1 << 20), who, ": size out of range");
@@ -1447,7 +1455,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
                     (o.stride(2) == 1 || W == 1),
                 who, ": out must look like q, with unit inner stride");
     at::assert_no_internal_overlap(o);
-    for (const Tensor* t : {&q, &k_pages, &v_pages}) at::assert_no_overlap(o, *t);
+    for (const Tensor* t : {&q, &k_pages, &v_pages}) check_apart(o, *t, who, "out and an input");
   } else {
     o = at::empty({N, nh, W}, q.options());
   }
@@ -1553,8 +1561,10 @@ Tensor penalize_logits(const Tensor& logits, const std::optional<Tensor>& tokens
                     (o.stride(1) == 1 || V == 1),
                 who, ": out must look like the logits, with unit inner stride");
     at::assert_no_internal_overlap(o);
-    if (bias.has_value()) at::assert_no_overlap(o, *bias);
-    at::assert_no_partial_overlap(o, logits);   // in place is fine: every element is read and written by one thread
+    if (bias.has_value()) check_apart(o, *bias, who, "out and bias");
+    // in place is fine: every element is read and written by one thread
+    if (o.data_ptr() != logits.data_ptr() || (R > 1 && o.stride(0) != logits.stride(0)))
+      check_apart(o, logits, who, "out and the logits, which are not the same tensor,");
   } else {
     o = at::empty({R, V}, logits.options());
   }

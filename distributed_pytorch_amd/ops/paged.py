@@ -128,7 +128,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     what the rows then hold is unspecified (nothing outside the buffers is touched).
 
     ``max_q``: an upper bound of the new tokens of a request, if the host knows one (a decode step: 1); it selects
-    kernels, not results. ``out``: the result's buffer; rows outside every request keep what it holds (without
+    kernels, not results. ``out``: the result's buffer, apart from the inputs; rows outside every request keep what it holds (without
     ``out`` they are zero)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])

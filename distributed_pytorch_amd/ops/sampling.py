@@ -85,7 +85,8 @@ def penalize_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, pr
       give token 0 for it.
 
     The penalties are numbers or fp32 tensors with one value or one per row, lengths int32 tensors likewise; they are
-    read by the kernel, so a captured step sees what a replay's buffers hold. ``out`` may be ``logits`` itself. No
+    read by the kernel, so a captured step sees what a replay's buffers hold. ``out`` may be ``logits`` itself,
+    but not overlap it otherwise. No
     gradients: on the GPU, tensors that require them are refused outside ``torch.no_grad()``."""
     if use_hip(logits):
         refuse_grad("penalize_logits", logits, repetition, presence, frequency, bias, out)
