@@ -24,15 +24,14 @@ CSRC = ROOT / "csrc"
 OBJ = ROOT / "build" / "obj"
 OUT = ROOT / "distributed_pytorch_amd" / "_C.so"
 ARCH = "gfx950"
+# Plain fp32 instructions only: some forms of the packed ones have given wrong results now and then, with no error. (The
+# host pass does not know the feature and says so.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Per-file code generation options. Keeping MFMA accumulators in architectural VGPRs avoids the
 # v_accvgpr_read/write traffic that VALU work on accumulators (softmax rescale, dS) otherwise pays.
-_NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # plain fp32 instructions only
 EXTRA_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-    "paged_plan.hip": _NO_PACKED_FP32,
-    "paged_append.hip": _NO_PACKED_FP32,
-    "paged_attn.hip": [*_NO_PACKED_FP32, "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-    "penalties.hip": _NO_PACKED_FP32,
+    "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 # Sources that textually include another source (rebuilt when that one changes).
 EXTRA_DEPS = {
@@ -84,7 +83,7 @@ def build(force: bool = False, asm: bool = False, verbose: bool = True) -> Path:
         obj = OBJ / (src.stem + ".o")
         objs.append(obj)
         if force or _stale(src, obj, headers + [CSRC / d for d in EXTRA_DEPS.get(src.name, [])]):
-            cmd = [hipcc, *common, *EXTRA_FLAGS.get(src.name, []), "-c", str(src), "-o", str(obj)]
+            cmd = [hipcc, *common, *NO_PACKED_FP32, *EXTRA_FLAGS.get(src.name, []), "-c", str(src), "-o", str(obj)]
             if asm:
                 (ROOT / "build" / "asm").mkdir(parents=True, exist_ok=True)
                 cmd += ["-save-temps=obj", "-Rpass-analysis=kernel-resource-usage"]

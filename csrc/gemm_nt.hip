@@ -125,7 +125,7 @@ __device__ __forceinline__ void barrier() {
 // Exact-erf GELU and its derivative. erfc by Abramowitz-Stegun 7.1.26 (|error| <= 1.5e-7):
 // Phi(-|x|) = 0.5 * t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2 / 2), t = 1 / (1 + p |x| / sqrt 2).
 #ifndef DPA_GELU_VARIANT
-#define DPA_GELU_VARIANT 2   // 0: one value at a time; 1: pairs in packed fp32 arithmetic; 2: pairs, sign by bit copy; 3: 2 + one reciprocal per pair
+#define DPA_GELU_VARIANT 2   // 0: one value at a time; 1: pairs; 2: pairs, sign by bit copy; 3: 2 + one reciprocal per pair
 #endif
 __device__ __forceinline__ void gelu_and_grad(float x, float& act, float& dact) {
   const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.3275911f * 0.70710678f, 1.0f));
@@ -140,7 +140,7 @@ __device__ __forceinline__ void gelu_and_grad(float x, float& act, float& dact) 
   dact = fmaf(x * e, 0.3989422804f, phi);
 }
 
-// The same on two values with the plain arithmetic in packed fp32 instructions (v_pk_fma_f32 / v_pk_mul_f32).
+// The same on two values at a time (in plain fp32 instructions: the build leaves the packed ones out).
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f32x2 splat2(float v) { return f32x2{v, v}; }
@@ -786,7 +786,7 @@ __global__ __launch_bounds__(512, 2) void gemm_nt_kernel(GemmNtArgs p) {
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              // (pairs in packed fp32 arithmetic: half the multiply / add instructions)
+              // (two values at a time)
               const f32x2 xa = {lo_bf16(x0[j]), hi_bf16(x0[j])}, xb = {lo_bf16(x1[j]), hi_bf16(x1[j])};
               f32x2 va = {v[2 * j], v[2 * j + 1]}, vb = {v[8 + 2 * j], v[8 + 2 * j + 1]};
               if (EPI == kEpiMul) {
@@ -802,7 +802,7 @@ __global__ __launch_bounds__(512, 2) void gemm_nt_kernel(GemmNtArgs p) {
             u32x4 o, hg, hu;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              // silu(g) * u on a pair of columns in packed fp32 arithmetic
+              // silu(g) * u on a pair of columns
               const f32x2 g = {v[2 * j], v[2 * j + 1]}, u = {v[8 + 2 * j], v[8 + 2 * j + 1]};
               const f32x2 z = g * splat2(-1.4426950408889634f);
               const f32x2 den = f32x2{__builtin_amdgcn_exp2f(z[0]), __builtin_amdgcn_exp2f(z[1])} + splat2(1.0f);
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(512, 2) void gemm_nt_kernel(GemmNtArgs p) {
             u32x4 dg0, dg1, du0, du1;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              // pairs in packed fp32 arithmetic: d(up) = ds g sg, d(gate) = ds u sg (1 + g (1 - sg)), sg = sigmoid(g)
+              // pairs: d(up) = ds g sg, d(gate) = ds u sg (1 + g (1 - sg)), sg = sigmoid(g)
               const f32x2 gs[2] = {{lo_bf16(g0[j]), hi_bf16(g0[j])}, {lo_bf16(g1[j]), hi_bf16(g1[j])}};
               const f32x2 us[2] = {{lo_bf16(u0[j]), hi_bf16(u0[j])}, {lo_bf16(u1[j]), hi_bf16(u1[j])}};
               const f32x2 ds[2] = {{v[2 * j], v[2 * j + 1]}, {v[8 + 2 * j], v[8 + 2 * j + 1]}};
