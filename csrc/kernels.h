@@ -353,7 +353,7 @@ struct PagedAttnArgs {
   FastDiv by_page;
   float scale;
   int window;        // 0: none
-  int max_q;         // no request has more new tokens (rows past it are left alone)
+  int max_q;         // a request has at most so many new tokens, as far as the host knows: selects kernels, not results
   int type;          // kTypeBf16 / kTypeHalf / kTypeFloat
   bool zero_rest;    // rows outside every sequence: true = zeroed, false = left as they are
 };

@@ -327,8 +327,8 @@ __device__ __forceinline__ Item find_item(const PagedAttnArgs& a, const FastArgs
 // ---- few rows only: equal shares of all steps ----
 // A (request, 32 packed rows, KV head) is a run of 128-key steps (one at least); the runs lie one after another, and workgroup i of `eff`
 // takes steps [i * per, (i + 1) * per) of them all, whichever runs they fall into: contexts of any mix of lengths load
-// the card evenly in one round. At most its first and its last run are cut.
-constexpr int kMinSteps = 1;           // steps worth a workgroup of their own (8 x 1k keys: 17.2 us; 2: 19.7, 4: 20.9, 8, uncut: 31.7)
+// the card evenly in one round. At most its first and its last run are cut. One step is worth a workgroup of its own (8 x
+// 1k keys: 17.2 us; two at least: 19.7, four: 20.9, eight, uncut: 31.7).
 
 struct Runs {        // the requests of the batch in LDS (R <= kWaveRequests)
   int before[kWaveRequests + 1];       // steps before each
@@ -395,7 +395,7 @@ __device__ __forceinline__ int find_run(const PagedAttnArgs& a, const FastArgs& 
 template <bool CHUNKS>
 __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a, FastArgs f) {
   __shared__ float red_f[16];
-  __shared__ int red_i[16], red_s[16], red_2[16];
+  __shared__ int red[3][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float cost = 0.f;
   bool back = false;
@@ -408,52 +408,53 @@ __global__ __launch_bounds__(1024) void paged_attn_items_kernel(PagedAttnArgs a,
   back = __syncthreads_or(back);
   if (tid == 0) f.header[3] = back;
   if (back) return;
-  const PieceSize size = piece_size(cost, a.nkv, f.target);
-  int base_i = 0, base_s = 0, base_2 = 0;
+  PieceSize size{};
+  if constexpr (CHUNKS) size = piece_size(cost, a.nkv, f.target);
+  // scans of the first items (few rows: steps), and for chunks of the second items and the slots
+  constexpr int NS = CHUNKS ? 3 : 1;
+  int* const out[3] = {f.prefix, f.prefix + 2 * (a.R + 1), f.prefix + a.R + 1};
+  int base[NS] = {};
   for (int r0 = 0; r0 < a.R; r0 += 1024) {
     const int r = r0 + tid;
-    int ni = 0, ns = 0, n2 = 0;
+    int n[NS] = {};
     if (r < a.R) {
       const Request q = request(a, f.G, r);
-      const int np = CHUNKS ? pieces(q, size) : 1;
-      ni = CHUNKS ? first_items(q, np, a.nkv) : run_steps(q) * run_count(q, a.nkv);
-      n2 = CHUNKS ? second_items(q, np, a.nkv) : 0;
-      ns = np > 1 ? ni + n2 : 0;
+      if constexpr (CHUNKS) {
+        const int np = pieces(q, size);
+        n[0] = first_items(q, np, a.nkv);
+        n[1] = second_items(q, np, a.nkv);
+        n[2] = np > 1 ? n[0] + n[1] : 0;
+      } else {
+        n[0] = run_steps(q) * run_count(q, a.nkv);
+      }
     }
-    int pi = wave_scan(ni), ps = wave_scan(ns), p2 = wave_scan(n2);
-    if (lane == 63) {
-      red_i[wave] = pi;
-      red_s[wave] = ps;
-      red_2[wave] = p2;
+    int p[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      p[i] = wave_scan(n[i]);
+      if (lane == 63) red[i][wave] = p[i];
     }
     __syncthreads();
-    int ti = 0, ts = 0, t2 = 0;
-    for (int w = 0; w < 16; ++w) {
-      if (w == wave) {
-        pi += ti;
-        ps += ts;
-        p2 += t2;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      int total = 0;
+      for (int w = 0; w < 16; ++w) {
+        if (w == wave) p[i] += total;
+        total += red[i][w];
       }
-      ti += red_i[w];
-      ts += red_s[w];
-      t2 += red_2[w];
+      if (r < a.R) out[i][r] = base[i] + p[i] - n[i];
+      base[i] += total;
     }
-    if (r < a.R) {
-      f.prefix[r] = base_i + pi - ni;
-      f.prefix[a.R + 1 + r] = base_s + ps - ns;
-      f.prefix[2 * (a.R + 1) + r] = base_2 + p2 - n2;
-    }
-    base_i += ti;
-    base_s += ts;
-    base_2 += t2;
     __syncthreads();
   }
   if (tid == 0) {
-    f.prefix[a.R] = base_i;
-    f.prefix[3 * a.R + 2] = base_2;
-    if (CHUNKS) f.header[0] = min(base_s, f.max_slots);
-    f.header[1] = size.few;
-    f.header[2] = size.chunk;
+    out[0][a.R] = base[0];
+    if constexpr (CHUNKS) {
+      out[1][a.R] = base[1];
+      f.header[0] = min(base[2], f.max_slots);
+      f.header[1] = size.few;
+      f.header[2] = size.chunk;
+    }
   }
 }
 
@@ -1110,7 +1111,7 @@ __global__ __launch_bounds__(kThreads, W == 64 ? 3 : 2) void paged_attn_few_kern
   __shared__ Runs runs;
   const int total = list_runs(a, f, runs);
   const int id = blockIdx.x;
-  const int eff = min((int)gridDim.x, max((total + kMinSteps - 1) / kMinSteps, 1));
+  const int eff = min((int)gridDim.x, max(total, 1));
   const int per = max((total + eff - 1) / eff, 1);
   if (id == 0 && tid == 0) f.header[0] = 2 * eff;
   if (id >= eff) return;

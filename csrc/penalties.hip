@@ -25,7 +25,6 @@ constexpr int kPenLds = 52 * 1024;        // counters of a workgroup: three work
 constexpr int kPenMin = 1024;             // entries below which a slice is not worth a workgroup
 constexpr int kPenUnroll = 4;
 
-template <typename T>
 __device__ __forceinline__ float penalized(float f, unsigned c, unsigned seen_bit, float rep, float freq, float pres) {
   if (c != 0u) {
     f = f > 0.f ? f / rep : f * rep;
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(kPenThreads) void penalties_kernel(PenaltyArgs a, i
       if (i >= n) break;
       if (total > 0) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[u][e] = penalized<T>(f[u][e], cnt[i * VEC + e], kSeen, rep, freq, pres);
+        for (int e = 0; e < VEC; ++e) f[u][e] = penalized(f[u][e], cnt[i * VEC + e], kSeen, rep, freq, pres);
       }
       if (bias != nullptr) {
 #pragma unroll
