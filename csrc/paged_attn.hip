@@ -123,12 +123,15 @@ __global__ __launch_bounds__(kGenWaves * 64) void paged_attn_rows_kernel(PagedAt
 // depend on which workgroup ran when. The second kernel costs 4 - 6 us of every call.
 //
 // Measured (large copy on the same card 4.9 TB/s, plain reads 6.2, a large bf16 product 1.48 PF/s):
-//   64 requests x 2000-8000 keys, 32 / 8 heads of 128, bf16      213 us   5.9 TB/s: the bytes
-//   2 requests x 33 K-131 K keys, same heads, fp16               105 us   5.8 TB/s
+//   64 requests x 2000-8000 keys, 32 / 8 heads of 128, bf16      215 us   5.9 TB/s: the bytes
+//   2 requests x 33 K-131 K keys, same heads, fp16               106 us   5.7 TB/s
 //   8 requests x 250-1000 keys, 12 heads of 64, bf16              17 us   four dependent trips to memory (lengths, table,
 //                                                                         keys, join) on a quarter-empty card
-//   8 prompts of 1000-3000 rows on 500-2000 cached, 32 / 8 x 128  640 us  0.86 PF/s: the LDS pipe (transposed reads) and
-//                                                                         the vector instructions of the softmax
+//   8 prompts of 1000-3000 rows on 500-2000 cached, 32 / 8 x 128  640 - 680 us  0.81 - 0.86 PF/s: the matrix pipes are
+//                                                                         busy 38 % of the time, the CUs hold waves 95 %
+//   8 prompts of 2048 rows, 16 heads of 64                       112 - 116 us  0.6 PF/s
+// The first form of a page's addresses that fits is taken (64 x 8000 keys of 128): whole runs of 16 rows in a page 230 us,
+// of 4 (pages of 20) 240, an address per lane (pages of 18) 260.
 //
 // Two things the loops live from, both found in the compiler's waits: nothing in them may spill (a reload is a
 // vector-memory wait, which waits for the transfers in flight: 737 -> 1232 us on the prompts), so what is rare is done
