@@ -966,7 +966,7 @@ class LLM(nn.Module):
         try:
             cfg = self.config
             fits = idx.size(1) + max_new_tokens - 1 <= cfg.block_size and max_new_tokens >= 3
-            able = idx.is_cuda and StaticKVCache.static_width(cfg) is not None and fits
+            able = idx.is_cuda and StaticKVCache.static_width(cfg) is not None and fits and ops.sample_captures(self.lm_head.weight)
             if hip_graph is None:
                 hip_graph = able
             self.last_decode_graphed = False      # introspection: did the last call replay a graph?
@@ -1106,7 +1106,7 @@ class LLM(nn.Module):
                 tok.copy_(sample(lg))
 
             left, graph = max_new_tokens - 1, None
-            if (history.is_cuda if hip_graph is None else hip_graph and history.is_cuda) and left >= 2:
+            if (hip_graph is None or hip_graph) and ops.sample_captures(self.lm_head.weight) and left >= 2:
                 step()                                       # lazy initialisations happen outside the capture
                 left -= 1
                 graph = torch.cuda.CUDAGraph()

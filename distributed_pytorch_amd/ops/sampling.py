@@ -30,11 +30,21 @@ def sample_eager(logits: torch.Tensor, temperature: float = 1.0, topk: int | Non
     return torch.multinomial(p, num_samples=1)
 
 
+_MAX_VOCAB = 57344      # of the kernel: a row stays in one workgroup's registers
+
+
 def _fused_ok(logits: torch.Tensor) -> bool:
     V = logits.shape[-1]
     return (use_hip(logits) and logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32)
-            and logits.stride(1) == 1 and V % 8 == 0 and 8 <= V <= 57344
+            and logits.stride(1) == 1 and V % 8 == 0 and 8 <= V <= _MAX_VOCAB
             and (logits.stride(0) * logits.element_size()) % 16 == 0 and logits.data_ptr() % 16 == 0)
+
+
+def sample_captures(weight: torch.Tensor) -> bool:
+    """Whether sampling from the logits of this head ``[V, C]`` may be part of a captured step: it is the kernel then. The
+    stock chain holds reductions over whole rows, which clear their semaphores with a memset, and such nodes have given
+    wrong results on replays."""
+    return use_hip(weight) and weight.shape[0] <= _MAX_VOCAB
 
 
 def sample_step_supported(logits: torch.Tensor) -> bool:
@@ -57,7 +67,15 @@ def sample_fused(logits: torch.Tensor, temperature: float = 1.0, topk: int | Non
     """Same distribution from one kernel launch, infinite logits included. ``seed``: int64 ``[1]`` on the device (default:
     drawn)."""
     if not _fused_ok(logits):
-        return sample_eager(logits, temperature, topk)
+        if not (use_hip(logits) and logits.dim() == 2 and logits.is_floating_point() and 1 <= logits.shape[1] <= _MAX_VOCAB):
+            return sample_eager(logits, temperature, topk)
+        # rows that the kernel's 16-byte loads cannot take (a vocabulary that is no multiple of 8, odd strides): a copy,
+        # filled up with logits of -inf, which are never drawn
+        B, V = logits.shape
+        dtype = torch.bfloat16 if logits.dtype == torch.bfloat16 else torch.float32
+        rows = torch.full((B, (V + 7) // 8 * 8), -float("inf"), dtype=dtype, device=logits.device)
+        rows[:, :V] = logits
+        logits = rows
     if seed is None:
         seed = torch.randint(-(1 << 62), 1 << 62, (1,), dtype=torch.int64, device=logits.device)
     return ops().sample_topk(logits, float(temperature), int(topk or 0), seed)

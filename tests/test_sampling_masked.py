@@ -136,3 +136,46 @@ def test_generation_under_a_mask_on_the_gpu(graph):
             assert m.last_decode_graphed == graph and set(out[:, 9:].unique().tolist()) <= may
             out = m.generate_ragged(list(idx), 40, topk=topk, hip_graph=graph, penalties=pen)
             assert m.last_decode_graphed == graph and set(torch.stack(out)[:, 9:].unique().tolist()) <= may
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1, 7, 97, 4099, 50257])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_fused_sampler_on_odd_vocabularies(V, dtype):
+    """Rows that 16-byte loads cannot take: the largest logit at top-1, the top-k set, the whole row without a filter."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = (torch.randn(40, V, device="cuda", generator=g) * 2).to(dtype)
+    tok = ops.sample_fused(x, 1.0, 1)
+    assert tok.shape == (40, 1) and torch.equal(x.gather(1, tok)[:, 0], x.amax(-1))
+    for k in (5, V):
+        kth = torch.topk(x.float(), min(k, V)).values[:, -1:]
+        for _ in range(20):
+            tok = ops.sample_fused(x, 0.7, k)
+            assert int(tok.max()) < V and (x.float().gather(1, tok) >= kth).all()
+    wide = torch.full((40, V + 3), 99.0, device="cuda").to(dtype)      # rows off 16 bytes inside a larger buffer
+    wide[:, 1:V + 1] = x
+    assert torch.equal(x.gather(1, ops.sample_fused(wide[:, 1:V + 1], 1.0, 1))[:, 0], x.amax(-1))
+    seed = torch.tensor([11], device="cuda")
+    assert torch.equal(ops.sample_fused(x, 0.7, None, seed), ops.sample_fused(wide[:, 1:V + 1], 0.7, None, seed))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,graphed", [(509, True), (50257, True), (57350, False)])
+def test_captured_generation_over_odd_vocabularies(V, graphed):
+    """Sampling is part of a captured step only as the kernel: a larger vocabulary decodes eagerly, with the same tokens."""
+    torch.manual_seed(0)
+    m = LLM(LLMconfig(vocab_size=V, block_size=64, n_embd=128, n_layer=1, n_head=2, up_dim=128, attn="mha", pos_emb="learn",
+                      non_linearity="gelu").finalize()).cuda().eval()    # fp32: bf16 logits tie, and ties are drawn
+    idx = torch.randint(0, V, (3, 5), device="cuda")
+    pen = dict(frequency=1e4)                      # no token twice: every step has to see the ones before it
+    want = m.generate_ragged(list(idx), 30, topk=1, hip_graph=False, penalties=pen)
+    got = m.generate_ragged(list(idx), 30, topk=1, penalties=pen)
+    assert m.last_decode_graphed == graphed
+    for a, b in zip(want, got):
+        assert torch.equal(a, b) and len(set(a[5:].tolist())) == 30
+    m.to(torch.bfloat16)                           # what the dense captured step takes
+    out = m.generate(idx, 30, topk=1, penalties=pen)
+    assert m.last_decode_graphed == graphed
+    assert all(len(set(row[5:].tolist())) == 30 and int(row.max()) < V for row in out)
+    free = m.generate_ragged(list(idx), 30, topk=20)
+    assert all(int(o.max()) < V and int(o.min()) >= 0 for o in free)
