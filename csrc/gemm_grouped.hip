@@ -254,6 +254,12 @@ __global__ __launch_bounds__(256, 2) void gemm_grouped_wgrad_kernel(GroupedWgrad
     }
 }
 
+// Zeros by a kernel, not a memset: a captured step holds this, and replays of memset nodes have gone wrong.
+__global__ __launch_bounds__(256) void zero_f32_kernel(f32x4* __restrict__ out, long long n4) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256)
+    out[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 void gemm_grouped_wgrad(const void* a, long long lda, const void* b, long long ldb, float* out,
                         const long long* seg_start, const long long* seg_rows, int ngroups, int N, int K,
                         int max_rows, hipStream_t st) {
@@ -275,7 +281,11 @@ void gemm_grouped_wgrad(const void* a, long long lda, const void* b, long long l
   if (splits > max_s) splits = max_s;
   if (splits < 1) splits = 1;
   p.splits = splits;
-  if (splits > 1) (void)hipMemsetAsync(out, 0, sizeof(float) * (size_t)ngroups * N * K, st);
+  if (splits > 1) {
+    const long long n4 = (long long)ngroups * N * K / 4;      // K % 128 == 0
+    const int blocks = (int)(n4 < 2048 * 256 ? (n4 + 255) / 256 : 2048);
+    hipLaunchKernelGGL(zero_f32_kernel, dim3(blocks), dim3(256), 0, st, (f32x4*)out, n4);
+  }
   const dim3 grid(tiles * splits, ngroups), block(256);
   static bool attr = false;
   if (!attr) {
