@@ -956,7 +956,8 @@ class LLM(nn.Module):
 
         ``hip_graph`` (default: automatic) decodes from ONE captured hipGraph per token over a
         preallocated cache when the model is on the GPU, its key rows fit the flash kernels (head size
-        64 / 128, or an MLA latent key of at most 128 columns) and prompt plus new tokens fit the context: a decode step is a few hundred small kernels, bound by launch cost.
+        64 / 128, or an MLA latent key of at most 128 columns), prompt plus new tokens fit the context and the
+        sampling kernel takes the vocabulary (57344 tokens): a decode step is a few hundred small kernels, bound by launch cost.
 
         ``penalties``: keyword arguments of ``ops.penalize_logits`` (``repetition``, ``presence``, ``frequency``, ``bias``,
         ``allowed``), applied to the logits of every step with the tokens so far as the history. Where they leave a row no
@@ -1066,7 +1067,8 @@ class LLM(nn.Module):
                         hip_graph: bool | None = None, penalties: dict | None = None, page_size: int = 16):
         """Sampling for prompts of different lengths in one batch: ``prompts`` (a list of 1-D token tensors) -> the list of
         prompts with ``max_new_tokens`` tokens each. The prompts are worked off packed, without padding, into a paged
-        cache; every further step is one token per request, by default replayed from a captured hipGraph on the GPU.
+        cache; every further step is one token per request, by default replayed from a captured hipGraph on the GPU (for
+        vocabularies that the sampling kernel takes, up to 57344 tokens).
         Prompt plus new tokens must fit the context. ``penalties`` as in ``generate``."""
         was_training = self.training
         self.eval()
