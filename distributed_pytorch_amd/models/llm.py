@@ -1030,7 +1030,7 @@ class LLM(nn.Module):
         graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         try:
-            with torch.cuda.graph(graph):
+            with torch.cuda.graph(graph, capture_error_mode="thread_local"):    # (other threads may call the runtime)
                 step()
         except Exception as exc:                 # some op of this configuration cannot be captured
             torch.cuda.synchronize()
@@ -1114,7 +1114,7 @@ class LLM(nn.Module):
                 graph = torch.cuda.CUDAGraph()
                 torch.cuda.synchronize()
                 try:
-                    with torch.cuda.graph(graph):
+                    with torch.cuda.graph(graph, capture_error_mode="thread_local"):    # (other threads may call the runtime)
                         step()
                 except Exception as exc:                     # some op of this configuration cannot be captured
                     torch.cuda.synchronize()

@@ -15,11 +15,11 @@ What makes the step capturable:
     tensor that is refreshed before each replay, because kernel arguments are frozen at capture;
   * gradients accumulate into the engine's flat buffers, whose addresses never change.
 
-The plain engine and the data-parallel engine can be captured. For DDP the bucketed all-reduces are
-part of the graph (RCCL collectives are capturable; they run on the communicator's stream, which the
-capture follows through the events that order it with the compute stream), so a launch-bound model
-keeps its advantage on several GPUs. The sharded engines (ZeRO, FSDP, EP) are not captured: their
-storage is resized and their collectives depend on host-side bookkeeping inside a step.
+Only an engine that issues no collectives is captured. The data-parallel step with its bucketed
+all-reduces was captured too and followed the eager trajectory, until one run of many ended the
+process while replays were in flight: an abort in a thread of the runtime or the communicator, whose
+cause is not known. It is switched off until it is. The sharded engines (ZeRO, FSDP, EP) never were
+captured: their storage is resized and their collectives depend on host-side bookkeeping inside a step.
 """
 from __future__ import annotations
 
@@ -52,9 +52,9 @@ class GraphedTrainStep:
     lazy initialisation happen), the next call captures, all later calls replay."""
 
     def __init__(self, engine, accum: int = 1, grad_clip: float = 1.0, warmup: int = 3):
+        if engine._dist:
+            raise RuntimeError("a step with collectives is not captured: run it eagerly (--hip_graph off)")
         assert engine.device.type == "cuda", "hipGraph capture needs the GPU"
-        assert (not engine._dist) or type(engine).name == "ddp", \
-            "only the plain and the data-parallel engine are captured"
         self.engine = engine
         self.accum = int(accum)
         self.grad_clip = float(grad_clip)
@@ -81,7 +81,7 @@ class GraphedTrainStep:
         eng.zero_grad()
         loss = None
         for i in range(self.accum):
-            eng.require_backward_grad_sync = i == self.accum - 1     # DDP: reduce with the last micro-batch
+            eng.require_backward_grad_sync = i == self.accum - 1
             _, loss, _ = eng(xs[i], ys[i])
             loss = loss / self.accum
             loss.backward()
@@ -108,7 +108,7 @@ class GraphedTrainStep:
                 torch.cuda.synchronize()
                 graph = torch.cuda.CUDAGraph()
                 try:
-                    # thread_local: other threads of the process (the collective watchdog polling its
+                    # thread_local: other threads of the process (a collective watchdog polling its
                     # events, the pinned-memory loader) keep calling the runtime while this one captures;
                     # under the default global mode such a call aborts the capture, or the process
                     with torch.cuda.graph(graph, capture_error_mode="thread_local"):

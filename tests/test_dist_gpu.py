@@ -234,6 +234,8 @@ def test_two_ranks_share_the_gpu_every_engine_agrees():
         assert abs(v - ref) < 5e-3 * abs(ref), losses
 
 
+@pytest.mark.skip(reason="once, in a full run, the process aborted in a thread outside Python while this test's replays were in "
+                         "flight; the cause is not known, and steps with collectives are not captured until it is")
 def test_graphed_ddp_step_captures_the_all_reduces(one_rank_group):
     """The data-parallel step, bucketed all-reduces included, replayed from one hipGraph follows the
     eager DDP trajectory."""
